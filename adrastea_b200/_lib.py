@@ -63,6 +63,15 @@ SIGNATURES = {
                              + [_vp, C.c_float]),
     "adr_decode_rope_attention": (_c_int, [_vp] * 8 + [_c_int] * 8 + [_vp, C.c_float, C.c_float]),
     "adr_attention_f16": (_c_int, [_vp] * 6 + [_c_int] * 5 + [_vp] * 4 + [C.c_float, C.c_uint32]),
+    "adr_rope_turns": (_c_int, [C.POINTER(C.c_uint64), C.POINTER(C.c_float), _c_int, C.c_double, C.c_uint32]
+                       + [C.c_double] * 4),
+    "adr_rope_f16": (_c_int, [_vp] * 4 + [_c_int] * 3 + [_vp] * 4 + [_c_int, C.c_float, C.c_uint32]),
+    "adr_rope_append_paged": (_c_int, [_vp] * 8 + [_c_int] * 5 + [_vp] * 9 + [_c_int] * 3
+                              + [_vp, _c_int, C.c_float, C.c_uint32]),
+    "adr_attention_packed": (_c_int, [_vp] * 6 + [_c_int] * 6 + [_vp] * 5 + [C.c_float, C.c_uint32]),
+    "adr_attention_paged_workspace": (C.c_size_t, [_vp] + [_c_int] * 3),
+    "adr_attention_paged": (_c_int, [_vp] * 6 + [_c_int] * 6 + [_vp] * 7 + [_c_int] * 3
+                            + [C.c_float, _vp, C.c_size_t]),
     "adr_allreduce_oneshot": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int,
                                        C.c_longlong, _c_int]),
     "adr_rms_norm_matmul_nt_fp16u8": (_c_int, [_vp, _vp, _vp, _vp, _vp, C.c_float, _vp, _vp, _vp,

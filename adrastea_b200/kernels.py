@@ -149,6 +149,63 @@ class MatmulOptions:
         return self
 
 
+class RopeLayout(enum.IntEnum):
+    """Which columns of a head make pair i of d rotated columns."""
+    Interleaved = 0  # (2i, 2i + 1), rotary.cu:4-29
+    Half = 1         # (i, i + d / 2)
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How the frequencies theta^(-2i/d) are changed for contexts `factor` times longer than the
+    `original` one (adr_rope_turns has the formulas)."""
+    kind: int = 0
+    factor: float = 1.0
+    original: float = 0.0
+    low: float = 0.0
+    high: float = 0.0
+
+    @staticmethod
+    def Identity() -> "RopeScaling":
+        return RopeScaling()
+
+    @staticmethod
+    def Linear(factor: float) -> "RopeScaling":
+        return RopeScaling(1, float(factor))
+
+    @staticmethod
+    def Base(factor: float) -> "RopeScaling":
+        return RopeScaling(2, float(factor))
+
+    @staticmethod
+    def Bands(factor: float, original: float, low: float = 1.0, high: float = 4.0) -> "RopeScaling":
+        return RopeScaling(3, float(factor), float(original), float(low), float(high))
+
+    @staticmethod
+    def Yarn(factor: float, original: float, high: float = 32.0, low: float = 1.0) -> "RopeScaling":
+        return RopeScaling(4, float(factor), float(original), float(low), float(high))
+
+
+def rope_turns(rotary_dim: int, theta: float, scaling: RopeScaling | None = None) -> tuple[list[int], float]:
+    """adr_rope_turns: (turns per position of each pair as fractions of 2^64, amplitude)."""
+    s = scaling or RopeScaling()
+    turns, amplitude = (C.c_uint64 * max(rotary_dim // 2, 1))(), C.c_float()
+    lib = _lib.load()
+    rc = lib.adr_rope_turns(turns, C.byref(amplitude), rotary_dim, theta, s.kind, s.factor, s.original, s.low, s.high)
+    if rc != 0:
+        raise AdrError(rc, lib.adr_strerror(rc).decode())
+    return list(turns), float(amplitude.value)
+
+
+@dataclass(frozen=True)
+class RopeTable:
+    """The frequencies of a rotation on the device (GpuKernels.rope_table)."""
+    turns: torch.Tensor  # int64 [rotary_dim / 2], the bits of adr_rope_turns
+    rotary_dim: int
+    layout: RopeLayout
+    amplitude: float
+
+
 def lower_matmul(output: TensorView, left: TensorView, right: TensorView,
                  options: MatmulOptions) -> tuple:
     """The marshalling of GpuKernels::matmul_f16 (kernels.rs:825-887).
@@ -629,6 +686,121 @@ class GpuKernels:
                                          q.data_ptr(), k.data_ptr(), v.data_ptr(), outer, inner,
                                          s_q, s_k, hd, lower(q), lower(k), lower(v), lower(out),
                                          float(scale), int(mask))
+        self._check(rc)
+
+    # -- requests of different lengths ---------------------------------------
+    def _stream_of(self, stream) -> int:
+        """The given stream, or the current one of the library's device."""
+        if stream is not None:
+            return _stream_handle(stream)
+        if torch.cuda.current_device() == self.device:
+            return _current_stream_handle()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _rows(self, v: TensorView, what: str, tokens: int, heads: int, head_dim: int):
+        """The token and head strides of a [tokens, heads, head_dim] fp16 view on this device."""
+        lay = v.layout
+        self._f16(v, what)
+        assert lay.dims == (tokens, heads, head_dim), f"{what} must be {(tokens, heads, head_dim)}, is {lay.dims}"
+        assert lay.strides[2] == 1 or head_dim == 1, f"the columns of {what} must follow one another"
+        assert v.device.type == "cuda" and v.device.index == self.device, f"{what} must be on cuda:{self.device}"
+        return (C.c_longlong * 2)(lay.strides[0], lay.strides[1])
+
+    def _pool(self, t: torch.Tensor, what: str, shape):
+        """The page, slot and head strides of a [pages, page_size, kv_heads, head_dim] fp16 tensor."""
+        if t.dtype is not torch.float16:
+            raise TypeError(f"{what} must be float16, got {t.dtype}")
+        assert t.shape == shape and t.stride(3) == 1, f"{what} must be {tuple(shape)} with unit column stride"
+        assert t.is_cuda and t.device.index == self.device, f"{what} must be on cuda:{self.device}"
+        return (C.c_longlong * 3)(t.stride(0), t.stride(1), t.stride(2))
+
+    def _ints(self, t: torch.Tensor, what: str, dtype=torch.int32):
+        """The address of a contiguous integer array on this device."""
+        if t.dtype is not dtype:
+            raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+        assert t.is_contiguous() and t.is_cuda and t.device.index == self.device, \
+            f"{what} must be contiguous and on cuda:{self.device}"
+        return t.data_ptr()
+
+    def rope_table(self, rotary_dim: int, theta: float, layout: RopeLayout = RopeLayout.Interleaved,
+                   scaling: RopeScaling | None = None) -> RopeTable:
+        """The table that rope_f16 and rope_append_paged take: made once, copied to the device."""
+        turns, amplitude = rope_turns(rotary_dim, theta, scaling)
+        t = torch.tensor(turns, dtype=torch.int64, device=torch.device("cuda", self.device))
+        return RopeTable(t, rotary_dim, RopeLayout(layout), amplitude)
+
+    def rope_f16(self, out: TensorView, input: TensorView, positions: torch.Tensor, table: RopeTable, stream=None):
+        """adr_rope_f16: the heads of every row of `input` ([tokens, heads, head_dim]) rotated at
+        positions[row] (int32, device).  `out` may be `input`."""
+        T, H, hd = input.layout.dims
+        so, si = self._rows(out, "output", T, H, hd), self._rows(input, "input", T, H, hd)
+        assert positions.shape == (T,)
+        rc = self._lib.adr_rope_f16(
+            self._ctx, self._stream_of(stream), out.data_ptr(), input.data_ptr(), T, H, hd, so, si,
+            self._ints(positions, "positions"), self._ints(table.turns, "the table", torch.int64), table.rotary_dim,
+            table.amplitude, int(table.layout))
+        self._check(rc)
+
+    def rope_append_paged(self, q_out: TensorView, q: TensorView, k: TensorView, v: TensorView,
+                          k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                          cu_q: torch.Tensor, kv_len: torch.Tensor, table: RopeTable, stream=None):
+        """adr_rope_append_paged: q of the new tokens rotated into q_out (which may be q), k rotated and
+        v copied into the pages [pages, page_size, kv_heads, head_dim] of their sequences."""
+        T, H, hd = q.layout.dims
+        n_pages, page_size, Hk, _ = k_pages.shape
+        n = kv_len.shape[0]
+        so, sq = self._rows(q_out, "q_out", T, H, hd), self._rows(q, "q", T, H, hd)
+        sk, sv = self._rows(k, "k", T, Hk, hd), self._rows(v, "v", T, Hk, hd)
+        shape = (n_pages, page_size, Hk, hd)
+        skp, svp = self._pool(k_pages, "k_pages", shape), self._pool(v_pages, "v_pages", shape)
+        assert block_table.dim() == 2 and block_table.shape[0] == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
+        rc = self._lib.adr_rope_append_paged(
+            self._ctx, self._stream_of(stream), q_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            k_pages.data_ptr(), v_pages.data_ptr(), T, n, H, Hk, hd, so, sq, sk, sv, skp, svp,
+            self._ints(block_table, "block_table"), self._ints(cu_q, "cu_q"), self._ints(kv_len, "kv_len"),
+            block_table.shape[1], page_size, n_pages, self._ints(table.turns, "the table", torch.int64),
+            table.rotary_dim, table.amplitude, int(table.layout))
+        self._check(rc)
+
+    def attention_packed(self, out: TensorView, q: TensorView, k: TensorView, v: TensorView, cu_q: torch.Tensor,
+                         max_q: int, scale: float, mask: MatmulMask = MatmulMask.Causal, stream=None):
+        """adr_attention_packed: attention of whole prompts, the rows cu_q[s]..cu_q[s + 1] - 1 of q and out
+        ([tokens, heads, head_dim]) and of k and v ([tokens, kv_heads, head_dim]) to a sequence; `max_q`
+        is the longest one's rows."""
+        T, H, hd = q.layout.dims
+        Hk = k.size(-2)
+        so, sq = self._rows(out, "output", T, H, hd), self._rows(q, "q", T, H, hd)
+        sk, sv = self._rows(k, "k", T, Hk, hd), self._rows(v, "v", T, Hk, hd)
+        assert cu_q.dim() == 1
+        rc = self._lib.adr_attention_packed(
+            self._ctx, self._stream_of(stream), out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), T,
+            cu_q.shape[0] - 1, max_q, H, Hk, hd, so, sq, sk, sv, self._ints(cu_q, "cu_q"), float(scale), int(mask))
+        self._check(rc)
+
+    def attention_paged_workspace(self, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor:
+        """A workspace for attention_paged of these heads (zero, as its first use wants it).  Calls that
+        overlap in time need one each."""
+        need = self._lib.adr_attention_paged_workspace(self._ctx, n_heads, n_kv_heads, head_dim)
+        return torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", self.device))
+
+    def attention_paged(self, out: TensorView, q: TensorView, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                        block_table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, max_q: int,
+                        scale: float, workspace: torch.Tensor, stream=None):
+        """adr_attention_paged: the new rows of every sequence over its pages, which hold their own k and
+        v already; row i of lq sees the positions up to kv_len - lq + i.  `max_q` is the largest lq."""
+        T, H, hd = q.layout.dims
+        n_pages, page_size, Hk, _ = k_pages.shape
+        n = kv_len.shape[0]
+        so, sq = self._rows(out, "output", T, H, hd), self._rows(q, "q", T, H, hd)
+        shape = (n_pages, page_size, Hk, hd)
+        skp, svp = self._pool(k_pages, "k_pages", shape), self._pool(v_pages, "v_pages", shape)
+        assert block_table.dim() == 2 and block_table.shape[0] == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
+        assert workspace.is_contiguous() and workspace.is_cuda and workspace.device.index == self.device
+        rc = self._lib.adr_attention_paged(
+            self._ctx, self._stream_of(stream), out.data_ptr(), q.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), T, n, max_q, H, Hk, hd, so, sq, skp, svp, self._ints(block_table, "block_table"),
+            self._ints(cu_q, "cu_q"), self._ints(kv_len, "kv_len"), block_table.shape[1], page_size, n_pages,
+            float(scale), workspace.data_ptr(), workspace.numel() * workspace.element_size())
         self._check(rc)
 
     def rms_norm_matmul_nt_fp16u8(self, output: torch.Tensor, lhs: torch.Tensor,

@@ -493,6 +493,111 @@ int adr_attention_f16(adr_ctx* ctx, adr_stream stream, void* out, const void* q,
                       const long long* strides_v, const long long* strides_o, float scale,
                       uint32_t mask_op);
 
+/* ------------------------------------------------------------------------
+ * Serving requests of different lengths (no counterpart in the reference, which runs one sequence
+ * at a time, llama.rs:426-427).  Three arrays in device memory describe the batch, so that a
+ * captured step can be replayed with other lengths:
+ *   cu_q [n_seqs + 1]  the rows of sequence s are cu_q[s] .. cu_q[s + 1] - 1 (not decreasing; a
+ *                      sequence may have none); rows of no sequence are neither read nor written;
+ *   kv_len [n_seqs]    positions of sequence s with its new rows, which are the last of them: row i
+ *                      of lq is at position kv_len[s] - lq + i;
+ *   block_table [n_seqs, max_pages]  position p lies in slot p % page_size of page
+ *                      block_table[s][p / page_size]; entries behind the last position are not read.
+ * k_pages and v_pages are pools of n_pages pages.  Tensors of rows are addressed as base +
+ * row * strides[0] + head * strides[1] + column, pools as base + page * strides[0] +
+ * slot * strides[1] + head * strides[2] + column (elements, 64-bit, not negative).  Query head h
+ * belongs to key head h / (n_heads / n_kv_heads).  What the arrays hold is checked on the device:
+ * rows are cut to `tokens`, lengths to max_pages * page_size, and a page outside the pool is not
+ * written and reads as zeros; each of the last two, and a row at a negative position, also sets the
+ * word behind adr_device_status.  A tensor may not overlap one that the same call writes, unless
+ * its entry says so; two sequences may share pages that neither writes.
+ * ------------------------------------------------------------------------ */
+
+/* Pairs of adr_rope_f16 and adr_rope_append_paged: columns (2i, 2i + 1), or (i, i + rotary_dim / 2). */
+enum { ADR_ROPE_INTERLEAVED = 0, ADR_ROPE_HALF = 1 };
+/*
+ * Frequencies f_i of pair i of d = rotary_dim columns, theta^(-2i/d) unless scaled for contexts
+ * `factor` times longer:
+ *   LINEAR  f / factor (positions stretched)
+ *   BASE    theta * factor^(d / (d - 2)) in the place of theta
+ *   BANDS   by the turns n = original * f / (2 pi) that a pair makes within the original context:
+ *           w f + (1 - w) f / factor, w = clamp((n - low) / (high - low), 0, 1)
+ *   YARN    (Peng et al. 2023): w f / factor + (1 - w) f, w = clamp((i - a) / (b - a), 0, 1), a and b the
+ *           pairs (rounded down, up) that make `high` and `low` turns; the rotated columns are
+ *           multiplied by 0.1 ln(factor) + 1
+ */
+enum {
+  ADR_ROPE_SCALE_NONE = 0,
+  ADR_ROPE_SCALE_LINEAR = 1,
+  ADR_ROPE_SCALE_BASE = 2,
+  ADR_ROPE_SCALE_BANDS = 3,
+  ADR_ROPE_SCALE_YARN = 4
+};
+
+/*
+ * Fills turns[rotary_dim / 2], HOST memory, with f_i / (2 pi) as fractions of 2^64, and
+ * *amplitude.  The caller copies the table to the device once.  Needs no GPU and no context.
+ * theta > 1, factor >= 1, original > 0 and 0 < low < high where the scaling uses them.
+ */
+int adr_rope_turns(uint64_t* turns, float* amplitude, int rotary_dim, double theta, uint32_t scaling,
+                   double factor, double original, double low, double high);
+
+/*
+ * adr_rotary for rows at any positions: rows of n_heads heads, pair (a, b) of row t becomes
+ * amplitude * (a cos - b sin, b cos + a sin) of the angle positions[t] * f_i, in fp32 with one
+ * rounding; columns from rotary_dim on are copied.  `turns` is device memory.  In place
+ * (out == in with the same strides) is allowed.  Any strides and alignment; 16-byte pieces where
+ * all rows, heads and parts of a head begin on one.  head_dim <= 256.
+ */
+int adr_rope_f16(adr_ctx* ctx, adr_stream stream, void* out, const void* in, int tokens, int n_heads,
+                 int head_dim, const long long* strides_o, const long long* strides_i,
+                 const int32_t* positions, const uint64_t* turns, int rotary_dim, float amplitude,
+                 uint32_t layout);
+
+/*
+ * adr_prefill_rope_append for a paged cache: every row's q rotated at its position into q_out (which
+ * may be q, with the same strides), its k rotated and its v copied into their slots of the pools.
+ * A row whose page is outside the pool or the table still has its q rotated.
+ */
+int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_out, const void* q, const void* k,
+                          const void* v, void* k_pages, void* v_pages, int tokens, int n_seqs,
+                          int n_heads, int n_kv_heads, int head_dim, const long long* strides_qo,
+                          const long long* strides_q, const long long* strides_k,
+                          const long long* strides_v, const long long* strides_kp,
+                          const long long* strides_vp, const int32_t* block_table, const int32_t* cu_q,
+                          const int32_t* kv_len, int max_pages, int page_size, int n_pages,
+                          const uint64_t* turns, int rotary_dim, float amplitude, uint32_t layout);
+
+/*
+ * Attention of whole prompts of different lengths: the rows of sequence s of q against the same
+ * rows of k and v, mask Causal hiding key x from row y when x > y.  Scores, maxima and sums are fp32
+ * (scale is not rounded), probabilities are rounded to fp16 for the product with v, the output
+ * once.  `max_q`: the longest sequence's rows; it chooses the kernel and does not change what is
+ * computed.  head_dim 64 or 128, n_heads a multiple of n_kv_heads and at most 64 times it,
+ * pointers 16-byte aligned, strides multiples of 8; else ADR_ERR_SHAPE.
+ */
+int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, const void* q, const void* k,
+                         const void* v, int tokens, int n_seqs, int max_q, int n_heads, int n_kv_heads,
+                         int head_dim, const long long* strides_o, const long long* strides_q,
+                         const long long* strides_k, const long long* strides_v, const int32_t* cu_q,
+                         float scale, uint32_t mask_op);
+
+/*
+ * Attention of the new rows over the paged cache, which holds their own k and v already: row i of
+ * lq of sequence s sees positions 0 .. kv_len[s] - lq + i; a row that sees none becomes zeros.
+ * Arithmetic, max_q and rules as in adr_attention_packed; page_size a power of two from 16 to 256.
+ * `workspace`: adr_attention_paged_workspace bytes of device memory, 16-byte aligned, zero before its
+ * first use; every call leaves it fit for the next.  Calls that overlap in time need one each.
+ */
+size_t adr_attention_paged_workspace(const adr_ctx* ctx, int n_heads, int n_kv_heads, int head_dim);
+int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, const void* q, const void* k_pages,
+                        const void* v_pages, int tokens, int n_seqs, int max_q, int n_heads,
+                        int n_kv_heads, int head_dim, const long long* strides_o,
+                        const long long* strides_q, const long long* strides_kp,
+                        const long long* strides_vp, const int32_t* block_table, const int32_t* cu_q,
+                        const int32_t* kv_len, int max_pages, int page_size, int n_pages, float scale,
+                        void* workspace, size_t workspace_bytes);
+
 /*
  * No counterpart in the reference (it has no multi-GPU path, llama.rs:28-29): one-shot
  * all-reduce (sum) of an fp16 vector over peer memory, for the row-split products of
