@@ -1,4 +1,6 @@
 // Attention over sequences of different lengths: the entry points, and a kernel that is right for every case.
+#include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "paged.cuh"
@@ -124,7 +126,7 @@ extern "C" int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, 
 
 extern "C" size_t adr_attention_paged_workspace(const adr_ctx* ctx, int n_heads, int n_kv_heads, int head_dim) {
   if (!ctx || check_heads(n_heads, n_kv_heads, head_dim) != ADR_OK) return 0;
-  return 16;
+  return attention_few_workspace(ctx, head_dim);
 }
 
 extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, const void* q, const void* k_pages,
@@ -178,5 +180,6 @@ extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, c
   }
   p.scale = scale;
   p.status = ctx->d_status;
-  return launch_simple(ctx, (cudaStream_t)stream, p);
+  return launch_attention_few(ctx, (cudaStream_t)stream, p, (int)std::min<long long>((long long)max_q * p.group, 64),
+                              INT_MAX, workspace);
 }

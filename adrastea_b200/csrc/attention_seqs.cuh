@@ -19,4 +19,22 @@ struct SeqAttention {
   unsigned int* status;
 };
 
+// A copy of `rows` slots of one head of a page: [64 columns, 1 head, rows, 1 page] of a pool with strides page, slot,
+// head.  (A dimension of one element is given a stride that the copy engine takes.)
+inline int pool_map(adr_ctx* ctx, CUtensorMap* map, const __half* base, const long long* s, const SeqAttention& a,
+                    int rows) {
+  const uint64_t dims[4] = {(uint64_t)a.head_dim, (uint64_t)a.n_kv_heads, (uint64_t)a.page_size, (uint64_t)a.n_pages};
+  const long long st[3] = {s[2], s[1], s[0]};
+  uint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (uint64_t)st[i] * 2 : (uint64_t)a.head_dim * 2;
+  const uint32_t box[4] = {64u, 1u, (uint32_t)rows, 1u};
+  return tma_get(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Kernels of a few rows per sequence (attention_few.cu): `rows` rows of a key head at most chooses the tile,
+// sequences with more than max_rows are passed over.
+size_t attention_few_workspace(const adr_ctx* ctx, int head_dim);
+int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int rows, int max_rows,
+                         void* workspace);
+
 }  // namespace adr
