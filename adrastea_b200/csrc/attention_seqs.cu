@@ -1,4 +1,4 @@
-// Attention over sequences of different lengths: the entry points, and a kernel that is right for every case.
+// Attention over sequences of different lengths: the entry points and the choice of a kernel.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -10,55 +10,7 @@ namespace adr {
 
 namespace {
 
-// One warp per (row, query head): the keys one after the other with a running maximum and sum.
-template <int HD>
-__global__ void __launch_bounds__(128) attention_seqs_simple_kernel(SeqAttention p) {
-  constexpr int PER = HD / 32;
-  pdl_wait_trigger();
-  const int t = blockIdx.x, lane = threadIdx.x & 31;
-  const int s = find_sequence(p.cu_q, p.n_seqs, t, lane);
-  if (s >= p.n_seqs) return;
-  const SeqSpan span = seq_span(p.cu_q, p.kv_len, s, p.tokens, p.max_pages * p.page_size, p.status);
-  if (t < span.q0 || t >= span.q0 + span.lq) return;
-  const int limit = p.causal ? max(0, span.lk - span.lq + (t - span.q0) + 1) : span.lk;
-  for (int h = threadIdx.x >> 5; h < p.n_heads; h += 4) {
-    const int kh = h / p.group;
-    const __half* q = p.q + t * p.sq[0] + h * p.sq[1] + lane * PER;
-    float qf[PER], o[PER], m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < PER; ++i) qf[i] = __half2float(q[i]), o[i] = 0.0f;
-    for (int j = 0; j < limit; ++j) {
-      long long ko, vo;
-      bool real = true;
-      if (p.block_table) {
-        const int page = __ldg(p.block_table + (long long)s * p.max_pages + j / p.page_size);
-        real = page >= 0 && page < p.n_pages;
-        if (!real) atomicOr(p.status, PAGED_BAD);
-        ko = page * p.sk[0] + (j % p.page_size) * p.sk[1] + kh * p.sk[2];
-        vo = page * p.sv[0] + (j % p.page_size) * p.sv[1] + kh * p.sv[2];
-      } else {
-        ko = (long long)(span.q0 + j) * p.sk[1] + kh * p.sk[2];
-        vo = (long long)(span.q0 + j) * p.sv[1] + kh * p.sv[2];
-      }
-      float x = 0.0f;
-      for (int i = 0; i < PER; ++i) x += real ? qf[i] * __half2float(p.k[ko + lane * PER + i]) : 0.0f;
-      for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      x *= p.scale;
-      const float mn = fmaxf(m, x), mu = mn == -INFINITY ? 0.0f : mn;
-      const float a = expf(m - mu), w = expf(x - mu);
-      l = l * a + w;
-      for (int i = 0; i < PER; ++i) o[i] = o[i] * a + (real ? w * __half2float(p.v[vo + lane * PER + i]) : 0.0f);
-      m = mn;
-    }
-    __half* dst = p.out + t * p.so[0] + h * p.so[1] + lane * PER;
-    for (int i = 0; i < PER; ++i) dst[i] = __float2half_rn(limit > 0 ? o[i] / l : 0.0f);
-  }
-}
-
-int launch_simple(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& p) {
-  if (p.head_dim == 64) attention_seqs_simple_kernel<64><<<p.tokens, 128, 0, stream>>>(p);
-  else attention_seqs_simple_kernel<128><<<p.tokens, 128, 0, stream>>>(p);
-  return after_launch(ctx);
-}
+constexpr int FEW_ROWS = 64;  // rows of a key head up to which the kernel of few rows takes a sequence
 
 // The strides of n dimensions of the given extents: not negative, and 16-byte steps where a dimension has more
 // than one element.
@@ -121,7 +73,7 @@ extern "C" int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, 
   }
   p.scale = scale;
   p.status = ctx->d_status;
-  return launch_simple(ctx, (cudaStream_t)stream, p);
+  return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1);
 }
 
 extern "C" size_t adr_attention_paged_workspace(const adr_ctx* ctx, int n_heads, int n_kv_heads, int head_dim) {
@@ -180,6 +132,10 @@ extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, c
   }
   p.scale = scale;
   p.status = ctx->d_status;
-  return launch_attention_few(ctx, (cudaStream_t)stream, p, (int)std::min<long long>((long long)max_q * p.group, 64),
-                              INT_MAX, workspace);
+  const long long rows = (long long)max_q * p.group;
+  if (rows <= FEW_ROWS) return launch_attention_few(ctx, (cudaStream_t)stream, p, (int)rows, INT_MAX, workspace);
+  // all sequences of one length: tiles for all; otherwise those of few rows go to the other kernel
+  if ((long long)n_seqs * max_q == tokens) return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1);
+  if (int rc = launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, FEW_ROWS + 1); rc != ADR_OK) return rc;
+  return launch_attention_few(ctx, (cudaStream_t)stream, p, FEW_ROWS, FEW_ROWS, workspace);
 }

@@ -37,4 +37,8 @@ size_t attention_few_workspace(const adr_ctx* ctx, int head_dim);
 int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int rows, int max_rows,
                          void* workspace);
 
+// Tiles of many rows (attention_tiles.cu): `max_q` chooses the tiles of a CTA, sequences with fewer than min_rows rows
+// of a key head are passed over.
+int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int max_q, int min_rows);
+
 }  // namespace adr

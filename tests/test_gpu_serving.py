@@ -313,15 +313,18 @@ def test_packed_large_scores(kernels, hd):
 
 
 def test_packed_wrong_spans_stay_inside(kernels):
-    """cu_q outside the rows or falling: rows are cut to those there are, nothing outside is touched."""
+    """cu_q outside the rows: the spans are cut to the rows there are, and nothing outside is touched; where it falls,
+    the sequence has no rows."""
     g = gen(2)
     T, H, hd = 100, 2, 64
-    q, k, v = half(g, T, H, hd), half(g, T, H, hd), half(g, T, H, hd)
-    out = torch.full_like(q, 2.0)
-    kernels.attention_packed(view(out), view(q), view(k), view(v), ints([-50, 30, 20, 20, 1000]), 100, 0.1)
+    store = half(g, 3, T + 20, H, hd)
+    q, k, v = store[:, 10:-10]
+    out = torch.full((T + 20, H, hd), 2.0, dtype=torch.float16, device="cuda")
+    kernels.attention_packed(view(out[10:-10]), view(q), view(k), view(v), ints([-50, 30, 20, 30, 1000]), 100, 0.1)
     kernels.device_status()
-    assert_close(out[:30], *attend(q[:30], k[:30], v[:30], 0.1, 1))
-    assert_close(out[30:], *[t[10:] for t in attend(q[20:], k[20:], v[20:], 0.1, 1)])
+    assert (out[:10] == 2.0).all() and (out[-10:] == 2.0).all()
+    assert_close(out[10:30], *[t[:20] for t in attend(q[:30], k[:30], v[:30], 0.1, 1)])
+    assert_close(out[40:-10], *attend(q[30:], k[30:], v[30:], 0.1, 1))
 
 
 # ------------------------------------------------------------------ paged attention
