@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
+import functools
 import json
 from dataclasses import dataclass, field
 from typing import Optional
@@ -240,10 +241,16 @@ try:
 
     def _current_stream_handle() -> int:
         return _cuda_getCurrentRawStream(_cuda_getDevice())
+
+    def _current_stream_of(device: int) -> int:
+        return _cuda_getCurrentRawStream(device)
 except ImportError:  # private functions: a PyTorch without them has the public way
 
     def _current_stream_handle() -> int:
         return torch.cuda.current_stream().cuda_stream
+
+    def _current_stream_of(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _stream_handle(stream) -> int:
@@ -252,6 +259,16 @@ def _stream_handle(stream) -> int:
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream
     return int(stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def _strides2(a: int, b: int):
+    return (C.c_longlong * 2)(a, b)
+
+
+@functools.lru_cache(maxsize=4096)
+def _strides3(a: int, b: int, c: int):
+    return (C.c_longlong * 3)(a, b, c)
 
 
 class GpuKernels:
@@ -690,35 +707,34 @@ class GpuKernels:
 
     # -- requests of different lengths ---------------------------------------
     def _stream_of(self, stream) -> int:
-        """The given stream, or the current one of the library's device."""
-        if stream is not None:
-            return _stream_handle(stream)
-        if torch.cuda.current_device() == self.device:
-            return _current_stream_handle()
-        return torch.cuda.current_stream(self.device).cuda_stream
+        """The given stream, or the current one of the library's device (whichever device is current)."""
+        return _current_stream_of(self.device) if stream is None else _stream_handle(stream)
 
-    def _rows(self, v: TensorView, what: str, tokens: int, heads: int, head_dim: int):
+    def _rows(self, v: TensorView, what: str, dims: tuple):
         """The token and head strides of a [tokens, heads, head_dim] fp16 view on this device."""
-        lay = v.layout
-        self._f16(v, what)
-        assert lay.dims == (tokens, heads, head_dim), f"{what} must be {(tokens, heads, head_dim)}, is {lay.dims}"
-        assert lay.strides[2] == 1 or head_dim == 1, f"the columns of {what} must follow one another"
-        assert v.device.type == "cuda" and v.device.index == self.device, f"{what} must be on cuda:{self.device}"
-        return (C.c_longlong * 2)(lay.strides[0], lay.strides[1])
+        lay, base = v.layout, v.base
+        if base.dtype is not torch.float16:
+            raise TypeError(f"{what} must be float16, got {base.dtype}")
+        assert lay.dims == dims, f"{what} must be {dims}, is {lay.dims}"
+        s0, s1, s2 = lay.strides
+        assert s2 == 1 or dims[2] == 1, f"the columns of {what} must follow one another"
+        assert base.get_device() == self.device, f"{what} must be on cuda:{self.device}"
+        return _strides2(s0, s1)
 
-    def _pool(self, t: torch.Tensor, what: str, shape):
+    def _pool(self, t: torch.Tensor, what: str, shape: tuple):
         """The page, slot and head strides of a [pages, page_size, kv_heads, head_dim] fp16 tensor."""
         if t.dtype is not torch.float16:
             raise TypeError(f"{what} must be float16, got {t.dtype}")
-        assert t.shape == shape and t.stride(3) == 1, f"{what} must be {tuple(shape)} with unit column stride"
-        assert t.is_cuda and t.device.index == self.device, f"{what} must be on cuda:{self.device}"
-        return (C.c_longlong * 3)(t.stride(0), t.stride(1), t.stride(2))
+        s0, s1, s2, s3 = t.stride()
+        assert t.shape == shape and s3 == 1, f"{what} must be {tuple(shape)} with unit column stride"
+        assert t.get_device() == self.device, f"{what} must be on cuda:{self.device}"
+        return _strides3(s0, s1, s2)
 
     def _ints(self, t: torch.Tensor, what: str, dtype=torch.int32):
         """The address of a contiguous integer array on this device."""
         if t.dtype is not dtype:
             raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
-        assert t.is_contiguous() and t.is_cuda and t.device.index == self.device, \
+        assert t.is_contiguous() and t.get_device() == self.device, \
             f"{what} must be contiguous and on cuda:{self.device}"
         return t.data_ptr()
 
@@ -732,8 +748,8 @@ class GpuKernels:
     def rope_f16(self, out: TensorView, input: TensorView, positions: torch.Tensor, table: RopeTable, stream=None):
         """adr_rope_f16: the heads of every row of `input` ([tokens, heads, head_dim]) rotated at
         positions[row] (int32, device).  `out` may be `input`."""
-        T, H, hd = input.layout.dims
-        so, si = self._rows(out, "output", T, H, hd), self._rows(input, "input", T, H, hd)
+        dims = T, H, hd = input.layout.dims
+        so, si = self._rows(out, "output", dims), self._rows(input, "input", dims)
         assert positions.shape == (T,)
         rc = self._lib.adr_rope_f16(
             self._ctx, self._stream_of(stream), out.data_ptr(), input.data_ptr(), T, H, hd, so, si,
@@ -746,19 +762,20 @@ class GpuKernels:
                           cu_q: torch.Tensor, kv_len: torch.Tensor, table: RopeTable, stream=None):
         """adr_rope_append_paged: q of the new tokens rotated into q_out (which may be q), k rotated and
         v copied into the pages [pages, page_size, kv_heads, head_dim] of their sequences."""
-        T, H, hd = q.layout.dims
-        n_pages, page_size, Hk, _ = k_pages.shape
-        n = kv_len.shape[0]
-        so, sq = self._rows(q_out, "q_out", T, H, hd), self._rows(q, "q", T, H, hd)
-        sk, sv = self._rows(k, "k", T, Hk, hd), self._rows(v, "v", T, Hk, hd)
-        shape = (n_pages, page_size, Hk, hd)
+        dims = T, H, hd = q.layout.dims
+        n_pages, page_size, Hk, _ = shape = k_pages.shape
+        n, kv = kv_len.shape[0], (T, Hk, hd)
+        so, sq = self._rows(q_out, "q_out", dims), self._rows(q, "q", dims)
+        sk, sv = self._rows(k, "k", kv), self._rows(v, "v", kv)
+        assert shape[3] == hd
         skp, svp = self._pool(k_pages, "k_pages", shape), self._pool(v_pages, "v_pages", shape)
-        assert block_table.dim() == 2 and block_table.shape[0] == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
+        seqs, max_pages = block_table.shape
+        assert seqs == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
         rc = self._lib.adr_rope_append_paged(
             self._ctx, self._stream_of(stream), q_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
             k_pages.data_ptr(), v_pages.data_ptr(), T, n, H, Hk, hd, so, sq, sk, sv, skp, svp,
             self._ints(block_table, "block_table"), self._ints(cu_q, "cu_q"), self._ints(kv_len, "kv_len"),
-            block_table.shape[1], page_size, n_pages, self._ints(table.turns, "the table", torch.int64),
+            max_pages, page_size, n_pages, self._ints(table.turns, "the table", torch.int64),
             table.rotary_dim, table.amplitude, int(table.layout))
         self._check(rc)
 
@@ -767,10 +784,10 @@ class GpuKernels:
         """adr_attention_packed: attention of whole prompts, the rows cu_q[s]..cu_q[s + 1] - 1 of q and out
         ([tokens, heads, head_dim]) and of k and v ([tokens, kv_heads, head_dim]) to a sequence; `max_q`
         is the longest one's rows."""
-        T, H, hd = q.layout.dims
-        Hk = k.size(-2)
-        so, sq = self._rows(out, "output", T, H, hd), self._rows(q, "q", T, H, hd)
-        sk, sv = self._rows(k, "k", T, Hk, hd), self._rows(v, "v", T, Hk, hd)
+        dims = T, H, hd = q.layout.dims
+        Hk = k.layout.dims[-2]
+        so, sq = self._rows(out, "output", dims), self._rows(q, "q", dims)
+        sk, sv = self._rows(k, "k", (T, Hk, hd)), self._rows(v, "v", (T, Hk, hd))
         assert cu_q.dim() == 1
         rc = self._lib.adr_attention_packed(
             self._ctx, self._stream_of(stream), out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), T,
@@ -788,18 +805,19 @@ class GpuKernels:
                         scale: float, workspace: torch.Tensor, stream=None):
         """adr_attention_paged: the new rows of every sequence over its pages, which hold their own k and
         v already; row i of lq sees the positions up to kv_len - lq + i.  `max_q` is the largest lq."""
-        T, H, hd = q.layout.dims
-        n_pages, page_size, Hk, _ = k_pages.shape
+        dims = T, H, hd = q.layout.dims
+        n_pages, page_size, Hk, _ = shape = k_pages.shape
         n = kv_len.shape[0]
-        so, sq = self._rows(out, "output", T, H, hd), self._rows(q, "q", T, H, hd)
-        shape = (n_pages, page_size, Hk, hd)
+        so, sq = self._rows(out, "output", dims), self._rows(q, "q", dims)
+        assert shape[3] == hd
         skp, svp = self._pool(k_pages, "k_pages", shape), self._pool(v_pages, "v_pages", shape)
-        assert block_table.dim() == 2 and block_table.shape[0] == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
-        assert workspace.is_contiguous() and workspace.is_cuda and workspace.device.index == self.device
+        seqs, max_pages = block_table.shape
+        assert seqs == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
+        assert workspace.is_contiguous() and workspace.get_device() == self.device
         rc = self._lib.adr_attention_paged(
             self._ctx, self._stream_of(stream), out.data_ptr(), q.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), T, n, max_q, H, Hk, hd, so, sq, skp, svp, self._ints(block_table, "block_table"),
-            self._ints(cu_q, "cu_q"), self._ints(kv_len, "kv_len"), block_table.shape[1], page_size, n_pages,
+            self._ints(cu_q, "cu_q"), self._ints(kv_len, "kv_len"), max_pages, page_size, n_pages,
             float(scale), workspace.data_ptr(), workspace.numel() * workspace.element_size())
         self._check(rc)
 
