@@ -11,6 +11,8 @@
 //     the keys take to arrive.)  With 16 rows the warps share a stage's keys, with 64 its rows.
 //   * An item that lies within one CTA is finished there.  Otherwise each part stores its maximum, sum and unscaled
 //     output, and the CTA that arrives last (a counter per border) joins the parts in their order: same bits each run.
+#include <algorithm>
+
 #include "attention_seqs.cuh"
 
 namespace adr {
@@ -29,14 +31,15 @@ struct FewCfg {
   static constexpr int CH = HD / 64;            // 64-column chunks of a head
   static constexpr int TILE = FEW_KB * HD * 2;  // bytes of a stage's keys
   static constexpr int STAGES = HD == 128 ? 3 : 6;
-  static constexpr int MERGE = 2 * (HD / 8) * 32 * 8;
-  static constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * TILE + MERGE + 4 * 16 * 8 + 16 * STAGES + 32;
+  static constexpr int MERGE = WK == 1 ? 0 : 4 * (HD / 8) * 32 * 8;  // eight rows of every warp
+  static constexpr size_t SMEM = (size_t)STAGES * 2 * TILE + MERGE + 4 * 16 * 8 + 16 * STAGES + 160;
 };
 
 struct FewParams {
   SeqAttention a;
   int max_rows;  // sequences with more rows of a key head than this are left to another kernel
   int page_rows; // rows of a copy: a page, 64 at most
+  int min_units; // of a CTA, where there are few
   float* part_ml;
   float* part_o;
   unsigned int* counters;
@@ -75,6 +78,17 @@ struct Walk {
   SeqSpan span;
   int s, head, tile, blk;
   int tiles, blks;
+};
+
+// How the units are shared out: CTA c begins with unit begin(c).
+struct Share {
+  long long per;
+  int ctas, more;
+  __device__ long long begin(int c) const { return c * per + min(c, more); }
+  __device__ int owner(long long u) const {
+    const long long big = more * (per + 1);
+    return u < big ? (int)(u / (per + 1)) : more + (int)((u - big) / per);
+  }
 };
 
 template <int ROWS>
@@ -151,13 +165,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
                          const __grid_constant__ FewParams p) {
   using Cfg = FewCfg<HD, WM>;
   constexpr int STAGES = Cfg::STAGES, WK = Cfg::WK, NT = HD / 8;
-  extern __shared__ uint8_t few_smem[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  float2* merge = reinterpret_cast<float2*>(ring + (size_t)STAGES * 2 * Cfg::TILE);   // [2][NT][32]
-  float2* ml = merge + 2 * NT * 32;                                                   // [4 warps][16 rows]
+  extern __shared__ __align__(1024) uint8_t few_smem[];  // (the swizzle's atoms begin on 1024 bytes)
+  uint8_t* ring = few_smem;
+  float2* merge = reinterpret_cast<float2*>(ring + (size_t)STAGES * 2 * Cfg::TILE);   // [4 warps][NT][32]
+  float2* ml = merge + Cfg::MERGE / 8;                                                // [4 warps][16 rows]
   uint64_t* full = reinterpret_cast<uint64_t*>(ml + 4 * 16);
   uint64_t* empty = full + STAGES;
-  unsigned int* flag = reinterpret_cast<unsigned int*>(empty + STAGES);
+  long long& s_total = *reinterpret_cast<long long*>(empty + STAGES);
+  volatile unsigned int& s_last = *reinterpret_cast<unsigned int*>(empty + STAGES + 1);
+  Walk* s_walk = reinterpret_cast<Walk*>(empty + STAGES + 2);  // [3]: the first item, then alternately the next ones
+  static_assert(sizeof(Walk) * 3 + 16 <= 160, "what a CTA's warps share");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -172,23 +189,27 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   pdl_wait_trigger();
 
   // One warp looks up what is to be done, so that the warps that meet at barriers agree on it whatever happens to
-  // the arrays meanwhile.  No more CTAs than units; CTA c has the units [total c / ctas, total (c + 1) / ctas).
-  __shared__ long long s_total;
-  __shared__ Walk s_walk[3];  // the first item, then alternately the next ones
+  // the arrays meanwhile.  No more CTAs than units; the first `total % ctas` CTAs have one unit more than the others.
   const FewWork<Cfg::ROWS> work(p);
+  auto share_of = [&](long long n) {
+    Share r;
+    r.ctas = (int)min((long long)gridDim.x, (n + p.min_units - 1) / p.min_units);
+    r.per = r.ctas ? n / r.ctas : 0;
+    r.more = (int)(n - r.per * r.ctas);
+    return r;
+  };
   if (warp == 0) {
-    const long long n = work.total(lane), c = min((long long)gridDim.x, n);
+    const long long n = work.total(lane);
+    const Share sh = share_of(n);
     Walk f = {};
-    if (blockIdx.x < c) f = work.find(n * blockIdx.x / c, lane);
+    if ((int)blockIdx.x < sh.ctas) f = work.find(sh.begin(blockIdx.x), lane);
     if (lane == 0) s_total = n, s_walk[2] = f;
   }
   __syncthreads();
-  const long long total = s_total;
+  const Share share = share_of(s_total);
   Walk w = s_walk[2];
-  const long long ctas = min((long long)gridDim.x, total);
-  if (blockIdx.x >= ctas || w.tiles == 0) return;
-  auto begin_of = [&](long long c) { return total * c / ctas; };
-  const long long u0 = begin_of(blockIdx.x), u1 = begin_of(blockIdx.x + 1);
+  if ((int)blockIdx.x >= share.ctas || w.tiles == 0) return;
+  const long long u0 = share.begin(blockIdx.x), u1 = share.begin(blockIdx.x + 1);
   bool ok = true;
 
   if (warp == 4) {
@@ -248,32 +269,41 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   // ldmatrix lane addresses inside a 64-column chunk: keys by keys (K), and transposed (V)
   const int k_key = ((lane >> 4) << 3) + (lane & 7), k_col = (lane >> 3) & 1;
   const int v_key = (((lane >> 3) & 1) << 3) + (lane & 7), v_col = lane >> 4;
-  int st = 0, turn = 0;
-  unsigned use = 0;
-  for (long long u = u0; u < u1;) {
-    const int first = w.blk, last = (int)min((long long)w.blks, w.blk + (u1 - u));
-    const int lk = w.span.lk, lq = w.span.lq, group = p.a.group;
-    const int live = min(Cfg::ROWS, lq * group - w.tile * Cfg::ROWS);  // rows of this tile
-    // the thread's two rows: their query rows, heads, and how many positions they see
-    int limit[2];
-    long long q_at[2], o_at[2];
+  // the thread's two rows of an item: how many positions they see, where their output goes; their queries
+  auto rows_of = [&](const Walk& x) { return min(Cfg::ROWS, x.span.lq * p.a.group - x.tile * Cfg::ROWS); };
+  auto enter = [&](const Walk& x, int (&limit)[2], __half* (&dst)[2], uint32_t (&qa)[HD / 16][4]) {
+    const __half* src[2];
+    const int live = rows_of(x);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = wm * 16 + quad + 8 * i;
-      const int rr = w.tile * Cfg::ROWS + min(r, live - 1);  // rows past the last repeat it and are not stored
-      const int tok = rr / group, h = w.head * group + rr - tok * group;
-      limit[i] = max(0, lk - lq + tok + 1);
-      q_at[i] = (long long)(w.span.q0 + tok) * p.a.sq[0] + h * p.a.sq[1];
-      o_at[i] = (long long)(w.span.q0 + tok) * p.a.so[0] + h * p.a.so[1];
+      const int r = x.tile * Cfg::ROWS + min(wm * 16 + quad + 8 * i, live - 1);  // rows past the last repeat it, unstored
+      const int tok = r / p.a.group, h = x.head * p.a.group + r - tok * p.a.group;
+      limit[i] = max(0, x.span.lk - x.span.lq + tok + 1);
+      src[i] = p.a.q + (long long)(x.span.q0 + tok) * p.a.sq[0] + h * p.a.sq[1];
+      dst[i] = p.a.out + (long long)(x.span.q0 + tok) * p.a.so[0] + h * p.a.so[1];
     }
-    // positions that every row of the tile sees (a smaller token sees fewer)
-    const int all_see = max(0, lk - lq + w.tile * Cfg::ROWS / group + 1);
-    uint32_t qa[HD / 16][4];
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        qa[kk][i] = *reinterpret_cast<const uint32_t*>(p.a.q + q_at[i & 1] + kk * 16 + (i >> 1) * 8 + pairc);
+        qa[kk][i] = *reinterpret_cast<const uint32_t*>(src[i & 1] + kk * 16 + (i >> 1) * 8 + pairc);
+  };
+  int st = 0, turn = 0, limit[2];
+  unsigned use = 0;
+  __half* dst[2];
+  uint32_t qa[HD / 16][4];
+  enter(w, limit, dst, qa);
+  for (long long u = u0;;) {
+    const int first = w.blk, last = (int)min((long long)w.blks, w.blk + (u1 - u));
+    const bool more = u + (last - first) < u1;
+    if (warp == 0 && more) {
+      Walk n = w;
+      work.next(n);
+      if (lane == 0) s_walk[turn] = n;
+    }
+    const int lk = w.span.lk, live = rows_of(w);
+    // positions that every row of the tile sees (an earlier token sees fewer)
+    const int all_see = max(0, lk - w.span.lq + w.tile * Cfg::ROWS / p.a.group + 1);
     float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -359,19 +389,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         // A probability of zero does not silence a value that is infinite or not a number.  Values behind the last
         // position (whatever the page holds there) are cleared; if one that only some rows see is not finite, the
         // step is done key by key, for the rows that see it.
-        uint32_t keep[2];
+        uint32_t keep[2], odd = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int key = key0 + pairc + 8 * i;
           keep[i] = (key < lk ? 0xFFFFu : 0u) | (key + 1 < lk ? 0xFFFF0000u : 0u);
         }
-        uint32_t odd = 0;
+        if (all_see < min(lk, key0 + 16)) {
 #pragma unroll 1
-        for (int d = 0; d < HD / 16; ++d) {
-          uint32_t vf[4];
-          ldsm_x4_t(v_addr(d), vf);
+          for (int d = 0; d < HD / 16; ++d) {
+            uint32_t vf[4];
+            ldsm_x4_t(v_addr(d), vf);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) odd |= not_finite2(vf[i] & keep[i & 1]);
+            for (int i = 0; i < 4; ++i) odd |= not_finite2(vf[i] & keep[i & 1]);
+          }
         }
         if (!__any_sync(0xffffffffu, odd != 0)) {
 #pragma unroll
@@ -409,23 +440,34 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       if (++st == STAGES) st = 0, ++use;
     }
 
-    // ---- the warps that shared the keys are joined ----
+    // ---- the warps that shared the keys agree on maximum and sum ----
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
+    if (WK > 1 && (lane & 3) == 0) {
+      ml[warp * 16 + quad] = make_float2(m[0], l[0]);
+      ml[warp * 16 + quad + 8] = make_float2(m[1], l[1]);
+    }
+    few_sync();
+    // the queries of the next item are on their way while this one is put together
+    int next_limit[2];
+    __half* next_dst[2];
+    Walk next_w = w;
+    if (more) {
+      next_w = s_walk[turn];
+      turn ^= 1;
+      if (next_w.tiles != 0) enter(next_w, next_limit, next_dst, qa);
+    }
     if constexpr (WK > 1) {
-      if ((lane & 3) == 0) {
-        ml[warp * 16 + quad] = make_float2(m[0], l[0]);
-        ml[warp * 16 + quad + 8] = make_float2(m[1], l[1]);
-      }
-      few_sync();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float top = -INFINITY, sum = 0.0f;
+#pragma unroll
         for (int j = 0; j < WK; ++j) top = fmaxf(top, ml[(wm * WK + j) * 16 + quad + 8 * i].x);
         const float um = top == -INFINITY ? 0.0f : top;
+#pragma unroll
         for (int j = 0; j < WK; ++j) {
           const float2 x = ml[(wm * WK + j) * 16 + quad + 8 * i];
           sum += x.y * exp2_fast(x.x - um);
@@ -436,133 +478,132 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         m[i] = top;
         l[i] = sum;
       }
-      // eight rows at a time; of four warps first 2 and 3 hand over to 0 and 1, then 1 to 0
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (wm * 16 + 8 * i >= live && WM == 1) continue;  // (the same for all warps)
-#pragma unroll
-        for (int half = WK / 2; half > 0; half >>= 1) {
-          float2* buf = merge + (WM == 1 ? wk % half : wm) * NT * 32 + lane;
-          if (wk >= half && wk < 2 * half) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) buf[t * 32] = make_float2(o[t][2 * i], o[t][2 * i + 1]);
-          }
-          few_sync();
-          if (wk < half) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              const float2 x = buf[t * 32];
-              o[t][2 * i] += x.x;
-              o[t][2 * i + 1] += x.y;
-            }
-          }
-          few_sync();
-        }
-      }
     }
 
     // ---- the item is finished here, or this part of it is put down ----
-    const long long i0 = u - first, i1 = i0 + w.blks;
     const bool whole = first == 0 && last == w.blks;
-    if (wk == 0) {
-      float* po = nullptr;
-      if (!whole) {
-        // a CTA has at most two parts: one that begins with its units, one that begins behind them
-        const size_t slot = 2 * (size_t)blockIdx.x + (u == u0 ? 0 : 1);
-        po = p.part_o + slot * (FEW_MAX_ROWS * HD);
-        float* pml = p.part_ml + slot * (FEW_MAX_ROWS * 2);
-        if ((lane & 3) == 0) {
+    // a CTA has at most two parts: one that begins with its units, one that begins behind them
+    const size_t slot = 2 * (size_t)blockIdx.x + (u == u0 ? 0 : 1);
+    float* po = p.part_o + slot * (FEW_MAX_ROWS * HD);
+    if (!whole && wk == 0 && (lane & 3) == 0) {
+      float2* pml = reinterpret_cast<float2*>(p.part_ml + slot * (FEW_MAX_ROWS * 2));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = wm * 16 + quad + 8 * i;
-            if (r < live) __stcg(reinterpret_cast<float2*>(pml) + r, make_float2(m[i], l[i]));
-          }
-        }
+      for (int i = 0; i < 2; ++i)
+        if (wm * 16 + quad + 8 * i < live) __stcg(pml + wm * 16 + quad + 8 * i, make_float2(m[i], l[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (WK > 1 && i > 0) {
+        if (WM == 1 && live <= 8) break;
+        few_sync();  // the first eight rows have been read
       }
+      if constexpr (WK > 1) {
+        float2* mine = merge + warp * NT * 32 + lane;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = wm * 16 + quad + 8 * i;
-        if (r >= live) continue;
-        // no visible position: zeros
-        const float inv = limit[i] > 0 ? 1.0f / l[i] : 0.0f;
+        for (int t = 0; t < NT; ++t) mine[t * 32] = make_float2(o[t][2 * i], o[t][2 * i + 1]);
+        few_sync();
+      }
+      const int r = wm * 16 + quad + 8 * i;
+      // no visible position: zeros
+      const float inv = limit[i] > 0 ? 1.0f / l[i] : 0.0f;
+      // every warp adds up and stores its share of the columns
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (whole) {
-            *reinterpret_cast<uint32_t*>(p.a.out + o_at[i] + t * 8 + pairc) = pack_half2(o[t][2 * i] * inv, o[t][2 * i + 1] * inv);
-          } else {
-            __stcg(reinterpret_cast<float2*>(po + r * HD + t * 8 + pairc), make_float2(o[t][2 * i], o[t][2 * i + 1]));
+      for (int tt = 0; tt < NT / WK; ++tt) {
+        const int t = WK > 1 ? wk * (NT / WK) + tt : tt;
+        float2 x = make_float2(0.0f, 0.0f);
+        if constexpr (WK > 1) {
+          const float2* from = merge + (wm * WK * NT + t) * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < WK; ++j) {
+            const float2 y = from[j * NT * 32];
+            x.x += y.x;
+            x.y += y.y;
           }
+        } else {
+          x = make_float2(o[tt][2 * i], o[tt][2 * i + 1]);
+        }
+        if (r < live) {
+          if (whole) *reinterpret_cast<uint32_t*>(dst[i] + t * 8 + pairc) = pack_half2(x.x * inv, x.y * inv);
+          else __stcg(reinterpret_cast<float2*>(po + r * HD + t * 8 + pairc), x);
         }
       }
     }
     if (!whole) {
-      // the CTAs that hold parts: from that of unit i0 to that of unit i1 - 1
-      auto cta_of = [&](long long x) {
-        long long c = x * ctas / total;
-        while (begin_of(c + 1) <= x) ++c;
-        while (begin_of(c) > x) --c;
-        return c;
-      };
-      const long long c0 = cta_of(i0), c1 = cta_of(i1 - 1);
+      // the CTAs that hold parts: from that of the item's first unit to that of its last
+      const long long i0 = u - first;
+      const int c0 = share.owner(i0), c1 = share.owner(i0 + w.blks - 1);
       __threadfence();
       few_sync();
       if (threadIdx.x == 0) {
-        const unsigned before = atomicAdd(p.counters + c0, 1u);
-        const bool is_last = before + 1 == (unsigned)(c1 - c0 + 1);
+        const bool is_last = atomicAdd(p.counters + c0, 1u) == (unsigned)(c1 - c0);
         if (is_last) p.counters[c0] = 0;  // as the next call finds it
         __threadfence();
-        *flag = is_last ? 1u : 0u;
+        s_last = is_last ? 1u : 0u;
       }
       few_sync();
-      if (*flag) {
-        // one row at a time to 32 threads, HD / 32 columns each
-        constexpr int PER = HD / 32;
+      if (s_last) {
+        // a row to a warp, HD / 32 columns to a lane; eight parts' loads in flight
+        constexpr int PER = HD / 32, DEEP = 8;
+        const int parts = c1 - c0 + 1;
+        const size_t slot0 = 2 * (size_t)c0 + (share.begin(c0) < i0 ? 1 : 0);  // the others are their CTAs' first
+        auto slot_of = [&](int j) { return j == 0 ? slot0 : 2 * (size_t)(c0 + j); };
         for (int r = warp; r < live; r += 4) {
           float top = -INFINITY;
-          for (long long c = c0 + lane; c <= c1; c += 32) {
-            const size_t slot = 2 * (size_t)c + (begin_of(c) >= i0 ? 0 : 1);
-            top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot * (FEW_MAX_ROWS * 2)) + r).x);
-          }
+          for (int j = lane; j < parts; j += 32)
+            top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_of(j) * (FEW_MAX_ROWS * 2)) + r).x);
           for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           const float um = top == -INFINITY ? 0.0f : top;
           float sum = 0.0f, acc[PER];
 #pragma unroll
           for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-          for (long long c = c0; c <= c1; ++c) {
-            const size_t slot = 2 * (size_t)c + (begin_of(c) >= i0 ? 0 : 1);
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot * (FEW_MAX_ROWS * 2)) + r);
-            const float f = exp2_fast(x.x - um);
-            const float* src = p.part_o + slot * (FEW_MAX_ROWS * HD) + r * HD + lane * PER;
-            sum += x.y * f;
-            if constexpr (PER == 4) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-              acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
-            } else {
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-              acc[0] += v.x * f, acc[1] += v.y * f;
+          for (int j0 = 0; j0 < parts; j0 += 32) {
+            float factor = 0.0f;
+            if (j0 + lane < parts) {
+              const float2 x = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_of(j0 + lane) * (FEW_MAX_ROWS * 2)) + r);
+              factor = exp2_fast(x.x - um);
+              sum += x.y * factor;
+            }
+            const int n = min(32, parts - j0);
+            for (int j = 0; j < n; j += DEEP) {
+              float4 v[DEEP];
+#pragma unroll
+              for (int d = 0; d < DEEP; ++d) {
+                v[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (j + d < n) {
+                  const float* src = p.part_o + slot_of(j0 + j + d) * (FEW_MAX_ROWS * HD) + r * HD + lane * PER;
+                  if constexpr (PER == 4) {
+                    v[d] = __ldcg(reinterpret_cast<const float4*>(src));
+                  } else {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+                    v[d].x = y.x, v[d].y = y.y;
+                  }
+                }
+              }
+#pragma unroll
+              for (int d = 0; d < DEEP; ++d) {
+                const float f = __shfl_sync(0xffffffffu, factor, j + d);
+                if (j + d >= n) break;
+                acc[0] += v[d].x * f, acc[1] += v[d].y * f;
+                if constexpr (PER == 4) acc[2] += v[d].z * f, acc[3] += v[d].w * f;
+              }
             }
           }
-          const int rr = w.tile * Cfg::ROWS + r, tok = rr / group;
-          const float inv = lk - lq + tok + 1 > 0 ? 1.0f / sum : 0.0f;
-          __half* dst = p.a.out + (long long)(w.span.q0 + tok) * p.a.so[0] + (w.head * group + rr - tok * group) * p.a.so[1] +
-                        lane * PER;
+          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          const int rr = w.tile * Cfg::ROWS + r, tok = rr / p.a.group;
+          const float inv = lk - w.span.lq + tok + 1 > 0 ? 1.0f / sum : 0.0f;
+          __half* at = p.a.out + (long long)(w.span.q0 + tok) * p.a.so[0] +
+                       (long long)(w.head * p.a.group + rr - tok * p.a.group) * p.a.so[1] + lane * PER;
 #pragma unroll
           for (int i = 0; i < PER; i += 2)
-            *reinterpret_cast<uint32_t*>(dst + i) = pack_half2(acc[i] * inv, acc[i + 1] * inv);
+            *reinterpret_cast<uint32_t*>(at + i) = pack_half2(acc[i] * inv, acc[i + 1] * inv);
         }
       }
     }
     u += last - first;
-    if (u >= u1) break;
-    if (warp == 0) {
-      work.next(w);
-      if (lane == 0) s_walk[turn] = w;
-    }
-    few_sync();  // (the flag has been read, too)
-    w = s_walk[turn];
-    turn ^= 1;
-    if (w.tiles == 0) break;
+    if (!more || next_w.tiles == 0) break;
+    w = next_w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) limit[i] = next_limit[i], dst[i] = next_dst[i];
   }
   if (!ok && lane == 0) atomicOr(p.a.status, 1u << 22);
 }
@@ -588,6 +629,7 @@ int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& 
   FewParams p;
   p.a = a;
   p.max_rows = max_rows;
+  p.min_units = std::max(1, ctx->tune_att_cs.load());
   p.page_rows = a.page_size < FEW_KB ? a.page_size : FEW_KB;
   const size_t g = few_ctas(ctx);
   p.counters = static_cast<unsigned int*>(workspace);
