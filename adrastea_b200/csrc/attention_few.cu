@@ -2,15 +2,20 @@
 //
 // The rows of one key head (its query heads times the new tokens, up to 64) share every key and value, so one pass
 // over the cache serves them all: what bounds this kernel is reading the cache once.
-//   * Work is counted in units of 64 keys of one (sequence, key head, tile of rows).  Every CTA computes from the
-//     lengths on the device where the 1/Gth part of all units that is its own begins, so the cache of a batch of very
-//     different lengths, or of one long sequence, is spread evenly over the SMs with no plan from the host.
-//   * A producer warp copies pages by TMA into a ring of stages (64 keys and values), across the borders of items.
+//   * Work is counted in units of 64 keys of one (sequence, key head, tile of rows) and cut into chunks by the lengths
+//     on the device, so the cache of a batch of very different lengths, or of one long sequence, is spread evenly with
+//     no plan from the host.  Every CTA has one chunk of its own, 80 % of an even share; the rest lies in small chunks
+//     that CTAs take as they get done (SMs do not get equal shares of the memory's bandwidth: with even shares the
+//     slowest of 296 CTAs was done after 94 us where the median one took 77).
+//   * The producer warp looks up what comes next and copies pages by TMA into a ring of stages (64 keys and values),
+//     across the borders of items.
 //   * Four warps compute: S = Q K^T and O += P V by mma.sync m16n8k16 with the 16 (32, 64) rows as M and a running
 //     maximum and sum.  (tcgen05 wants 64 or 128 rows: at up to 16 live ones the tensor work is 5 % of the time that
 //     the keys take to arrive.)  With 16 rows the warps share a stage's keys, with 64 its rows.
-//   * An item that lies within one CTA is finished there.  Otherwise each part stores its maximum, sum and unscaled
-//     output, and the CTA that arrives last (a counter per border) joins the parts in their order: same bits each run.
+//   * An item that lies within one chunk is finished there.  Otherwise each part stores its maximum, sum and unscaled
+//     output, and a second kernel, which is resident before the first one ends, joins them in their order.  (Joined by
+//     the CTA that came last, 111 parts took 65 us: a join is a chain of loads of about a microsecond each, and one CTA
+//     has too few of them in flight.)  What is cut where does not depend on who computes it: same bits each run.
 #include <algorithm>
 
 #include "attention_seqs.cuh"
@@ -21,7 +26,6 @@ namespace {
 
 constexpr int FEW_KB = 64;          // keys of a stage, and of a unit of work
 constexpr int FEW_THREADS = 160;    // four computing warps and the producer
-constexpr int FEW_MAX_ROWS = 64;
 
 template <int HD, int WM>
 struct FewCfg {
@@ -32,17 +36,24 @@ struct FewCfg {
   static constexpr int TILE = FEW_KB * HD * 2;  // bytes of a stage's keys
   static constexpr int STAGES = HD == 128 ? 3 : 6;
   static constexpr int MERGE = WK == 1 ? 0 : 4 * (HD / 8) * 32 * 8;  // eight rows of every warp
-  static constexpr size_t SMEM = (size_t)STAGES * 2 * TILE + MERGE + 4 * 16 * 8 + 16 * STAGES + 160;
+  static constexpr int SEGS = STAGES + 2;       // descriptors in flight (a segment has at least one stage)
+  static constexpr size_t SMEM = (size_t)STAGES * 2 * TILE + MERGE + 4 * 16 * 8 + 16 * STAGES + 8 * SEGS +
+                                 SEGS * 48;
+  static constexpr int SPARE = WM == 1 ? 2 : 1; // small chunks per CTA
 };
+
+struct Segment;
 
 struct FewParams {
   SeqAttention a;
   int max_rows;  // sequences with more rows of a key head than this are left to another kernel
   int page_rows; // rows of a copy: a page, 64 at most
   int min_units; // of a CTA, where there are few
-  float* part_ml;
-  float* part_o;
-  unsigned int* counters;
+  int spare, spare_units;  // small chunks per CTA where a share has at least spare_units units
+  float* part_ml;          // [slots][ROWS][2]: two slots to a chunk
+  float* part_o;           // [slots][ROWS][head_dim]
+  unsigned int* queue;     // small chunks taken so far; then the number of chunks of the call
+  Segment* begins;  // the first segment of every chunk
 };
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -70,31 +81,91 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 // Nonzero if one of the two halves is infinite or not a number (its exponent bits are all ones: adding one to them
 // carries into the sign, which was masked away).
 __device__ __forceinline__ uint32_t not_finite2(uint32_t x) { return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
-// The computing warps only.
+// The computing warps only: a barrier, and one that says whether the predicate holds for all of them.
 __device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool few_all(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
+      "barrier.cta.red.and.pred b, 1, 128, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+      : "=r"(r) : "r"((uint32_t)x) : "memory");
+  return r != 0;
+}
 
-// Where in the list of all units (sequence by sequence, key head by key head, tile by tile, 64 keys each) a CTA is.
+// Where in the list of all units (sequence by sequence, key head by key head, tile by tile, 64 keys each) one is.
 struct Walk {
   SeqSpan span;
   int s, head, tile, blk;
   int tiles, blks;
 };
 
-// How the units are shared out: CTA c begins with unit begin(c).
+// How the units are cut: the list is divided evenly into `ctas` spans, each of which is a CTA's own chunk and `spare`
+// small ones behind it.  Chunk 0 .. ctas - 1 are the CTAs' own, ctas + c * spare + i the small ones of span c.
 struct Share {
-  long long per;
-  int ctas, more;
-  __device__ long long begin(int c) const { return c * per + min(c, more); }
-  __device__ int owner(long long u) const {
-    const long long big = more * (per + 1);
-    return u < big ? (int)(u / (per + 1)) : more + (int)((u - big) / per);
+  int total, ctas, spare;
+  int per, more;      // units of a span (the first `more` spans have one more)
+  __device__ int span_begin(int c) const { return c * per + min(c, more); }
+  __device__ int own(int size) const { return spare ? size - size / 5 : size; }
+  __device__ int2 range(int chunk) const {
+    if (chunk < ctas) {
+      const int b = span_begin(chunk);
+      return make_int2(b, b + own(span_begin(chunk + 1) - b));
+    }
+    const int c = (chunk - ctas) / spare, i = chunk - ctas - c * spare;
+    const int b = span_begin(c), e = span_begin(c + 1), first = b + own(e - b), rest = e - first;
+    return make_int2(first + rest * i / spare, first + rest * (i + 1) / spare);
+  }
+  // the place of unit u's chunk in the order of the units: 1 + spare chunks to a span
+  __device__ int place(int u) const {
+    const int big = more * (per + 1);
+    const int c = u < big ? u / (per + 1) : more + (u - big) / per;
+    const int b = span_begin(c), size = span_begin(c + 1) - b, first = own(size);
+    int at = u - b, i = 0;
+    if (at >= first) {
+      const int rest = size - first;
+      at -= first;
+      while (i < spare - 1 && at >= rest * (i + 1) / spare) ++i;
+      ++i;
+    }
+    return c * (1 + spare) + i;
+  }
+  __device__ int place_of(int chunk) const {
+    if (chunk < ctas) return chunk * (1 + spare);
+    const int c = (chunk - ctas) / spare;
+    return c * (1 + spare) + 1 + chunk - ctas - c * spare;
   }
 };
+
+// A run of units of one item, as the producer hands it to the computing warps.
+struct Segment {
+  int q0, lq, lk;           // of the sequence
+  int head, tile;
+  int first, last, blks;    // blocks of this run, of the item; blks == 0: there is no more
+  int slot;                 // where a part goes (slots are in the order of the units)
+  int place0, parts;        // places of the item's parts
+  int slot0;                // slot of the first one; the others are the first slots of their places
+};
+static_assert(sizeof(Segment) == 48, "");
 
 template <int ROWS>
 struct FewWork {
   const FewParams& p;
-  __device__ explicit FewWork(const FewParams& p_) : p(p_) {}
+  const int lane, q;  // a lane stands for q sequences
+  int before, upto;   // units before and up to the end of its sequences
+  __device__ FewWork(const FewParams& p_, int lane_) : p(p_), lane(lane_), q((p_.a.n_seqs + 31) / 32) {
+    int mine = 0;
+#pragma unroll 4
+    for (int i = 0; i < q; ++i) mine += units(lane * q + i);
+    upto = scan(mine);
+    before = upto - mine;
+  }
+  __device__ int scan(int x) const {
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += o;
+    }
+    return x;
+  }
   __device__ SeqSpan span(int s) const {
     return seq_span(p.a.cu_q, p.a.kv_len, s, p.a.tokens, p.a.max_pages * p.a.page_size, p.a.status);
   }
@@ -103,17 +174,19 @@ struct FewWork {
     return rows > p.max_rows ? 0 : (int)((rows + ROWS - 1) / ROWS);
   }
   __device__ static int blocks(const SeqSpan& v) { return max(1, (v.lk + FEW_KB - 1) / FEW_KB); }
-  __device__ long long units(int s) const {
+  __device__ int units(int s) const {
     if (s >= p.a.n_seqs) return 0;
     const SeqSpan v = span(s);
-    return (long long)tiles(v) * blocks(v) * p.a.n_kv_heads;
+    return tiles(v) * blocks(v) * p.a.n_kv_heads;
   }
-  // by a whole warp
-  __device__ long long total(int lane) const {
-    long long n = 0;
-    for (int s = lane; s < p.a.n_seqs; s += 32) n += units(s);
-    for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
-    return n;
+  __device__ Share share() const {
+    Share r;
+    r.total = __shfl_sync(0xffffffffu, upto, 31);
+    r.ctas = min((int)gridDim.x, (r.total + p.min_units - 1) / p.min_units);
+    r.per = r.ctas ? r.total / r.ctas : 0;
+    r.more = r.total - r.per * r.ctas;
+    r.spare = r.per >= max(p.spare_units, 5 * p.spare) ? p.spare : 0;  // (no small chunk may be empty)
+    return r;
   }
   __device__ void enter(Walk& w, int s) const {
     w.s = s;
@@ -121,30 +194,38 @@ struct FewWork {
     w.tiles = tiles(w.span);
     w.blks = blocks(w.span);
   }
-  // Unit u of all, by a whole warp.  (The loops over sequences end behind the last one whatever the arrays hold; no
-  // tiles: there is no such unit.)
-  __device__ Walk find(long long u, int lane) const {
+  // Unit u of all, by the whole warp.  (The loops over sequences end behind the last one whatever happens to the arrays
+  // meanwhile; no tiles: there is no such unit.)
+  __device__ Walk find(int u) const {
     Walk w = {};
-    for (int s0 = 0; s0 < p.a.n_seqs; s0 += 32) {
-      const long long mine = units(s0 + lane);
-      long long upto = mine;
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += o;
+    const unsigned m = __ballot_sync(0xffffffffu, u < upto);
+    if (!m) return w;
+    const int l = __ffs(m) - 1;
+    u -= __shfl_sync(0xffffffffu, before, l);
+    int s = l * q;
+    if (q > 1) {
+      const int end = min(p.a.n_seqs, s + q);
+      for (;; s += 32) {
+        if (s >= end) return w;
+        const int mine = s + lane < end ? units(s + lane) : 0;
+        const int sum = scan(mine);
+        const unsigned h = __ballot_sync(0xffffffffu, u < sum);
+        if (h) {
+          const int f = __ffs(h) - 1;
+          u -= __shfl_sync(0xffffffffu, sum - mine, f);
+          s += f;
+          break;
+        }
+        u -= __shfl_sync(0xffffffffu, sum, 31);
       }
-      const unsigned m = __ballot_sync(0xffffffffu, u < upto);
-      if (m) {
-        const int l = __ffs(m) - 1;
-        const long long rest = u - __shfl_sync(0xffffffffu, upto - mine, l);
-        enter(w, s0 + l);
-        w.head = (int)(rest / ((long long)w.tiles * w.blks));
-        const int in_head = (int)(rest - (long long)w.head * w.tiles * w.blks);
-        w.tile = in_head / w.blks;
-        w.blk = in_head - w.tile * w.blks;
-        return w;
-      }
-      u -= __shfl_sync(0xffffffffu, upto, 31);
     }
+    enter(w, s);
+    if (w.tiles == 0) return w;
+    const int per_head = w.tiles * w.blks;
+    w.head = u / per_head;
+    const int in_head = u - w.head * per_head;
+    w.tile = in_head / w.blks;
+    w.blk = in_head - w.tile * w.blks;
     return w;
   }
   // the item behind w's; no tiles: there is none
@@ -159,6 +240,99 @@ struct FewWork {
   }
 };
 
+// Joins parts.  Block j stands for the border before chunk j: if an item goes across it, the blocks of its borders share
+// its rows.  Few parts: a row to a warp; many: a row to the block, the parts shared out among its warps.  All loads of
+// eight parts are in flight at once.  (What is read here was written by the launch before, or, if that gave up, is left
+// from another call: nothing is stored outside the rows there are.)
+constexpr int JOIN_THREADS = 128;
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(JOIN_THREADS) few_join_kernel(const __grid_constant__ FewParams p) {
+  constexpr int PER = HD / 32, DEEP = 8, WARPS = JOIN_THREADS / 32;
+  __shared__ float part[WARPS][HD];
+  __shared__ float2 part_ml[WARPS];
+  pdl_wait_trigger();
+  const int j = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.a.group;
+  const int n = (int)min(p.queue[1], gridDim.x + 1);
+  const Segment g = p.begins[j];
+  if (j >= n || g.first == 0) return;  // no item goes across
+  const int border = j - 1 - g.place0;
+  if (border < 0 || g.place0 < 0 || g.parts < 2 || border > g.parts - 2 || g.place0 + g.parts > n ||
+      g.slot0 >> 1 != g.place0)
+    return;
+  const int live = min(ROWS, g.lq * group - g.tile * ROWS);
+  const bool many = g.parts > DEEP;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  for (int r = many ? border : border * WARPS + warp; r < live; r += (g.parts - 1) * (many ? 1 : WARPS)) {
+    float m = -INFINITY, l = 0.0f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+    const int step = many ? WARPS : 1;
+    for (int j0 = many ? warp : 0; j0 < g.parts; j0 += DEEP * step) {
+      float2 x[DEEP];
+      float4 v[DEEP];
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d) {
+        const int at = j0 + d * step;
+        const size_t row = (size_t)(at == 0 ? g.slot0 : 2 * (g.place0 + min(at, g.parts - 1))) * ROWS + r;
+        x[d] = __ldcg(ml + row);
+        if constexpr (PER == 4) {
+          v[d] = __ldcg(reinterpret_cast<const float4*>(p.part_o + row * HD + lane * PER));
+        } else {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(p.part_o + row * HD + lane * PER));
+          v[d] = make_float4(y.x, y.y, 0.0f, 0.0f);
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d) {
+        if (j0 + d * step >= g.parts) x[d] = make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, x[d].x);
+      }
+      const float um = top == -INFINITY ? 0.0f : top, alpha = exp2_fast(m - um);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] *= alpha;
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d) {
+        if (j0 + d * step >= g.parts) break;
+        const float f = exp2_fast(x[d].x - um);
+        l += x[d].y * f;
+        acc[0] += v[d].x * f, acc[1] += v[d].y * f;
+        if constexpr (PER == 4) acc[2] += v[d].z * f, acc[3] += v[d].w * f;
+      }
+      m = top;
+    }
+    if (many) {
+      __syncthreads();  // (the row before has been read)
+      if (lane == 0) part_ml[warp] = make_float2(m, l);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) part[warp][lane * PER + i] = acc[i];
+      __syncthreads();
+      if (warp != 0) continue;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part_ml[w].x);
+      const float um = top == -INFINITY ? 0.0f : top;
+      l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = exp2_fast(part_ml[w].x - um);
+        l += part_ml[w].y * f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] += part[w][lane * PER + i] * f;
+      }
+    }
+    const int rr = g.tile * ROWS + r, tok = rr / group, row = g.q0 + tok, head = g.head * group + rr - tok * group;
+    if (row < 0 || row >= p.a.tokens || head < 0 || head >= p.a.n_heads) continue;
+    const float inv = g.lk - g.lq + tok + 1 > 0 ? 1.0f / l : 0.0f;
+    __half* at = p.a.out + (long long)row * p.a.so[0] + (long long)head * p.a.so[1] + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) *reinterpret_cast<uint32_t*>(at + i) = pack_half2(acc[i] * inv, acc[i + 1] * inv);
+  }
+}
+
 template <int HD, int WM>
 __global__ void __launch_bounds__(FEW_THREADS, 2)
     attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -171,10 +345,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   float2* ml = merge + Cfg::MERGE / 8;                                                // [4 warps][16 rows]
   uint64_t* full = reinterpret_cast<uint64_t*>(ml + 4 * 16);
   uint64_t* empty = full + STAGES;
-  long long& s_total = *reinterpret_cast<long long*>(empty + STAGES);
-  volatile unsigned int& s_last = *reinterpret_cast<unsigned int*>(empty + STAGES + 1);
-  Walk* s_walk = reinterpret_cast<Walk*>(empty + STAGES + 2);  // [3]: the first item, then alternately the next ones
-  static_assert(sizeof(Walk) * 3 + 16 <= 160, "what a CTA's warps share");
+  uint64_t* seg_full = empty + STAGES;                              // [SEGS]
+  Segment* segs = reinterpret_cast<Segment*>(seg_full + Cfg::SEGS);  // [SEGS]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -184,79 +356,101 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 4);
     }
+    for (int i = 0; i < Cfg::SEGS; ++i) mbar_init(&seg_full[i], 1);
     mbar_fence_init();
   }
-  pdl_wait_trigger();
-
-  // One warp looks up what is to be done, so that the warps that meet at barriers agree on it whatever happens to
-  // the arrays meanwhile.  No more CTAs than units; the first `total % ctas` CTAs have one unit more than the others.
-  const FewWork<Cfg::ROWS> work(p);
-  auto share_of = [&](long long n) {
-    Share r;
-    r.ctas = (int)min((long long)gridDim.x, (n + p.min_units - 1) / p.min_units);
-    r.per = r.ctas ? n / r.ctas : 0;
-    r.more = (int)(n - r.per * r.ctas);
-    return r;
-  };
-  if (warp == 0) {
-    const long long n = work.total(lane);
-    const Share sh = share_of(n);
-    Walk f = {};
-    if ((int)blockIdx.x < sh.ctas) f = work.find(sh.begin(blockIdx.x), lane);
-    if (lane == 0) s_total = n, s_walk[2] = f;
-  }
   __syncthreads();
-  const Share share = share_of(s_total);
-  Walk w = s_walk[2];
-  if ((int)blockIdx.x >= share.ctas || w.tiles == 0) return;
-  const long long u0 = share.begin(blockIdx.x), u1 = share.begin(blockIdx.x + 1);
+  pdl_wait_trigger();
   bool ok = true;
 
   if (warp == 4) {
     // ------------------------------- producer -------------------------------
+    // It alone looks up what is to be done, so that the warps that meet at barriers agree on it.
+    const FewWork<Cfg::ROWS> work(p, lane);
+    const Share share = work.share();
     const int pr = p.page_rows, page_size = p.a.page_size;
-    int st = 0;
+    int st = 0, issued = 0, seg = 0;
     unsigned use = 0;
-    long long issued = 0;
-    for (long long u = u0; u < u1;) {
-      const int last = (int)min((long long)w.blks, w.blk + (u1 - u));
-      const int* row = p.a.block_table + (long long)w.s * p.a.max_pages;
-      for (int b = w.blk; b < last; ++b) {
-        const int keys = min(FEW_KB, w.span.lk - b * FEW_KB);
-        if (keys <= 0) break;  // a sequence without positions
-        const int copies = (keys + pr - 1) / pr;
-        const int pos = b * FEW_KB + lane * pr;
-        int page = 0;
-        if (lane < copies) {
-          page = __ldg(row + pos / page_size);
-          if (page < 0 || page >= p.a.n_pages) {
-            page = p.a.n_pages;  // outside the map: zeros arrive
-            atomicOr(p.a.status, PAGED_BAD);
-          }
-        }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (use & 1u) ^ 1u));
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(&full[st], (unsigned)(copies * pr * HD * 2 * 2));
-        __syncwarp();
-        if (lane < copies) {
-          uint8_t* k_sm = ring + (size_t)st * 2 * Cfg::TILE + lane * pr * 128;
-          const int slot = pos % page_size;
-#pragma unroll
-          for (int c = 0; c < Cfg::CH; ++c) {
-            tma_load_4d(k_sm + c * FEW_KB * 128, &map_k, c * 64, w.head, slot, page, &full[st]);
-            tma_load_4d(k_sm + Cfg::TILE + c * FEW_KB * 128, &map_v, c * 64, w.head, slot, page, &full[st]);
-          }
-        }
-        ++issued;
-        if (++st == STAGES) st = 0, ++use;
+    auto publish = [&](const Segment& g) {
+      if (lane == 0) {
+        segs[seg % Cfg::SEGS] = g;
+        mbar_arrive(&seg_full[seg % Cfg::SEGS]);
       }
-      if (!ok) break;
-      u += last - w.blk;
-      if (u < u1) work.next(w);
-      if (w.tiles == 0) break;
+      ++seg;
+    };
+    auto wait_empty = [&] { return ok && __all_sync(0xffffffffu, mbar_wait(&empty[st], (use & 1u) ^ 1u)); };
+    if (blockIdx.x == 0 && lane == 0) p.queue[1] = (unsigned)(share.ctas * (1 + share.spare));
+    for (int chunk = blockIdx.x; chunk < share.ctas * (1 + share.spare);) {
+      const int2 range = share.range(chunk);
+      const int place = share.place_of(chunk);
+      Walk w = {};
+      if (range.x < range.y) w = work.find(range.x);
+      for (int u = range.x; u < range.y && w.tiles != 0 && ok;) {
+        const int last = min(w.blks, w.blk + range.y - u);
+        Segment g;
+        g.q0 = w.span.q0, g.lq = w.span.lq, g.lk = w.span.lk;
+        g.head = w.head, g.tile = w.tile;
+        g.first = w.blk, g.last = last, g.blks = w.blks;
+        // a chunk has at most two parts: one that begins with it, one that begins behind its beginning
+        g.slot = 2 * place + (u == range.x ? 0 : 1);
+        g.place0 = place, g.parts = 1, g.slot0 = g.slot;
+        if (w.blk != 0 || last != w.blks) {
+          const int i0 = u - w.blk;
+          g.place0 = share.place(i0);
+          g.parts = share.place(i0 + w.blks - 1) - g.place0 + 1;
+          if (w.blk != 0) {
+            const int before_i0 = i0 > 0 ? share.place(i0 - 1) : -1;
+            g.slot0 = 2 * g.place0 + (before_i0 == g.place0 ? 1 : 0);
+          }
+        }
+        publish(g);
+        if (u == range.x && lane == 0) p.begins[place] = g;
+        const int* row = p.a.block_table + (long long)w.s * p.a.max_pages;
+        for (int b = w.blk; b < last; ++b) {
+          const int keys = min(FEW_KB, w.span.lk - b * FEW_KB);
+          const int copies = (max(keys, 0) + pr - 1) / pr;  // none: a sequence without positions
+          const int pos = b * FEW_KB + lane * pr;
+          int page = 0;
+          if (lane < copies) {
+            page = __ldg(row + pos / page_size);
+            if (page < 0 || page >= p.a.n_pages) {
+              page = p.a.n_pages;  // outside the map: zeros arrive
+              atomicOr(p.a.status, PAGED_BAD);
+            }
+          }
+          ok = wait_empty();
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(&full[st], (unsigned)(copies * pr * HD * 2 * 2));
+          __syncwarp();
+          if (lane < copies) {
+            uint8_t* k_sm = ring + (size_t)st * 2 * Cfg::TILE + lane * pr * 128;
+            const int slot = pos % page_size;
+#pragma unroll
+            for (int c = 0; c < Cfg::CH; ++c) {
+              tma_load_4d(k_sm + c * FEW_KB * 128, &map_k, c * 64, w.head, slot, page, &full[st]);
+              tma_load_4d(k_sm + Cfg::TILE + c * FEW_KB * 128, &map_v, c * 64, w.head, slot, page, &full[st]);
+            }
+          }
+          ++issued;
+          if (++st == STAGES) st = 0, ++use;
+        }
+        u += last - w.blk;
+        if (u < range.y) work.next(w);
+      }
+      // The next chunk.  Every CTA with a chunk of its own asks until there is none, so that the queue has come round
+      // to zero when all have.
+      if (share.spare == 0) break;
+      unsigned taken = 0;
+      const unsigned n = (unsigned)(share.ctas * share.spare);
+      if (lane == 0) taken = atomicInc(p.queue, n + share.ctas - 1);
+      taken = __shfl_sync(0xffffffffu, taken, 0);
+      if (taken >= n) break;
+      chunk = share.ctas + (int)taken;
     }
+    Segment end = {};
+    publish(end);
     // every copy has landed before the CTA may end
-    for (long long i = max(0LL, issued - STAGES); i < issued; ++i)
+    for (int i = max(0, issued - STAGES); i < issued; ++i)
       if (!mbar_wait(&full[i % STAGES], (unsigned)(i / STAGES) & 1u)) ok = false;
     if (!ok && lane == 0) atomicOr(p.a.status, 1u << 21);
     return;
@@ -270,17 +464,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   const int k_key = ((lane >> 4) << 3) + (lane & 7), k_col = (lane >> 3) & 1;
   const int v_key = (((lane >> 3) & 1) << 3) + (lane & 7), v_col = lane >> 4;
   // the thread's two rows of an item: how many positions they see, where their output goes; their queries
-  auto rows_of = [&](const Walk& x) { return min(Cfg::ROWS, x.span.lq * p.a.group - x.tile * Cfg::ROWS); };
-  auto enter = [&](const Walk& x, int (&limit)[2], __half* (&dst)[2], uint32_t (&qa)[HD / 16][4]) {
+  auto rows_of = [&](const Segment& x) { return min(Cfg::ROWS, x.lq * p.a.group - x.tile * Cfg::ROWS); };
+  auto enter = [&](const Segment& x, int (&limit)[2], __half* (&dst)[2], uint32_t (&qa)[HD / 16][4]) {
     const __half* src[2];
     const int live = rows_of(x);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = x.tile * Cfg::ROWS + min(wm * 16 + quad + 8 * i, live - 1);  // rows past the last repeat it, unstored
       const int tok = r / p.a.group, h = x.head * p.a.group + r - tok * p.a.group;
-      limit[i] = max(0, x.span.lk - x.span.lq + tok + 1);
-      src[i] = p.a.q + (long long)(x.span.q0 + tok) * p.a.sq[0] + h * p.a.sq[1];
-      dst[i] = p.a.out + (long long)(x.span.q0 + tok) * p.a.so[0] + h * p.a.so[1];
+      limit[i] = max(0, x.lk - x.lq + tok + 1);
+      src[i] = p.a.q + (long long)(x.q0 + tok) * p.a.sq[0] + h * p.a.sq[1];
+      dst[i] = p.a.out + (long long)(x.q0 + tok) * p.a.so[0] + h * p.a.so[1];
     }
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk)
@@ -288,29 +482,28 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       for (int i = 0; i < 4; ++i)
         qa[kk][i] = *reinterpret_cast<const uint32_t*>(src[i & 1] + kk * 16 + (i >> 1) * 8 + pairc);
   };
-  int st = 0, turn = 0, limit[2];
+  int st = 0, seg = 0, limit[2];
   unsigned use = 0;
   __half* dst[2];
   uint32_t qa[HD / 16][4];
-  enter(w, limit, dst, qa);
-  for (long long u = u0;;) {
-    const int first = w.blk, last = (int)min((long long)w.blks, w.blk + (u1 - u));
-    const bool more = u + (last - first) < u1;
-    if (warp == 0 && more) {
-      Walk n = w;
-      work.next(n);
-      if (lane == 0) s_walk[turn] = n;
-    }
-    const int lk = w.span.lk, live = rows_of(w);
+  ok = mbar_wait(&seg_full[0], 0);
+  if (!few_all(ok)) {
+    if (threadIdx.x == 0) atomicOr(p.a.status, 1u << 22);
+    return;
+  }
+  Segment w = segs[0];
+  if (w.blks != 0) enter(w, limit, dst, qa);
+  while (w.blks != 0) {
+    const int lk = w.lk, live = rows_of(w);
     // positions that every row of the tile sees (an earlier token sees fewer)
-    const int all_see = max(0, lk - w.span.lq + w.tile * Cfg::ROWS / p.a.group + 1);
+    const int all_see = max(0, lk - w.lq + w.tile * Cfg::ROWS / p.a.group + 1);
     float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
 
-    for (int b = first; b < last && lk > 0; ++b) {
+    for (int b = w.first; b < w.last; ++b) {  // (without positions: one empty stage)
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[st], use & 1u));
       const uint32_t k_sm = smem_u32(ring + (size_t)st * 2 * Cfg::TILE);
       const uint32_t v_sm = k_sm + Cfg::TILE;
@@ -450,16 +643,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       ml[warp * 16 + quad] = make_float2(m[0], l[0]);
       ml[warp * 16 + quad + 8] = make_float2(m[1], l[1]);
     }
-    few_sync();
+    ++seg;
+    if (ok) ok = mbar_wait(&seg_full[seg % Cfg::SEGS], (unsigned)(seg / Cfg::SEGS) & 1u);
+    ok = few_all(ok);  // (all warps go on, or none does)
+    if (!ok) break;
     // the queries of the next item are on their way while this one is put together
     int next_limit[2];
     __half* next_dst[2];
-    Walk next_w = w;
-    if (more) {
-      next_w = s_walk[turn];
-      turn ^= 1;
-      if (next_w.tiles != 0) enter(next_w, next_limit, next_dst, qa);
-    }
+    const Segment next_w = segs[seg % Cfg::SEGS];
+    if (next_w.blks != 0) enter(next_w, next_limit, next_dst, qa);
     if constexpr (WK > 1) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -481,12 +673,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
     }
 
     // ---- the item is finished here, or this part of it is put down ----
-    const bool whole = first == 0 && last == w.blks;
-    // a CTA has at most two parts: one that begins with its units, one that begins behind them
-    const size_t slot = 2 * (size_t)blockIdx.x + (u == u0 ? 0 : 1);
-    float* po = p.part_o + slot * (FEW_MAX_ROWS * HD);
+    const bool whole = w.first == 0 && w.last == w.blks;
+    float* po = p.part_o + (size_t)w.slot * (Cfg::ROWS * HD);
     if (!whole && wk == 0 && (lane & 3) == 0) {
-      float2* pml = reinterpret_cast<float2*>(p.part_ml + slot * (FEW_MAX_ROWS * 2));
+      float2* pml = reinterpret_cast<float2*>(p.part_ml) + (size_t)w.slot * Cfg::ROWS;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (wm * 16 + quad + 8 * i < live) __stcg(pml + wm * 16 + quad + 8 * i, make_float2(m[i], l[i]));
@@ -528,79 +718,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         }
       }
     }
-    if (!whole) {
-      // the CTAs that hold parts: from that of the item's first unit to that of its last
-      const long long i0 = u - first;
-      const int c0 = share.owner(i0), c1 = share.owner(i0 + w.blks - 1);
-      __threadfence();
-      few_sync();
-      if (threadIdx.x == 0) {
-        const bool is_last = atomicAdd(p.counters + c0, 1u) == (unsigned)(c1 - c0);
-        if (is_last) p.counters[c0] = 0;  // as the next call finds it
-        __threadfence();
-        s_last = is_last ? 1u : 0u;
-      }
-      few_sync();
-      if (s_last) {
-        // a row to a warp, HD / 32 columns to a lane; eight parts' loads in flight
-        constexpr int PER = HD / 32, DEEP = 8;
-        const int parts = c1 - c0 + 1;
-        const size_t slot0 = 2 * (size_t)c0 + (share.begin(c0) < i0 ? 1 : 0);  // the others are their CTAs' first
-        auto slot_of = [&](int j) { return j == 0 ? slot0 : 2 * (size_t)(c0 + j); };
-        for (int r = warp; r < live; r += 4) {
-          float top = -INFINITY;
-          for (int j = lane; j < parts; j += 32)
-            top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_of(j) * (FEW_MAX_ROWS * 2)) + r).x);
-          for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          const float um = top == -INFINITY ? 0.0f : top;
-          float sum = 0.0f, acc[PER];
-#pragma unroll
-          for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
-          for (int j0 = 0; j0 < parts; j0 += 32) {
-            float factor = 0.0f;
-            if (j0 + lane < parts) {
-              const float2 x = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_of(j0 + lane) * (FEW_MAX_ROWS * 2)) + r);
-              factor = exp2_fast(x.x - um);
-              sum += x.y * factor;
-            }
-            const int n = min(32, parts - j0);
-            for (int j = 0; j < n; j += DEEP) {
-              float4 v[DEEP];
-#pragma unroll
-              for (int d = 0; d < DEEP; ++d) {
-                v[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (j + d < n) {
-                  const float* src = p.part_o + slot_of(j0 + j + d) * (FEW_MAX_ROWS * HD) + r * HD + lane * PER;
-                  if constexpr (PER == 4) {
-                    v[d] = __ldcg(reinterpret_cast<const float4*>(src));
-                  } else {
-                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
-                    v[d].x = y.x, v[d].y = y.y;
-                  }
-                }
-              }
-#pragma unroll
-              for (int d = 0; d < DEEP; ++d) {
-                const float f = __shfl_sync(0xffffffffu, factor, j + d);
-                if (j + d >= n) break;
-                acc[0] += v[d].x * f, acc[1] += v[d].y * f;
-                if constexpr (PER == 4) acc[2] += v[d].z * f, acc[3] += v[d].w * f;
-              }
-            }
-          }
-          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          const int rr = w.tile * Cfg::ROWS + r, tok = rr / p.a.group;
-          const float inv = lk - w.span.lq + tok + 1 > 0 ? 1.0f / sum : 0.0f;
-          __half* at = p.a.out + (long long)(w.span.q0 + tok) * p.a.so[0] +
-                       (long long)(w.head * p.a.group + rr - tok * p.a.group) * p.a.so[1] + lane * PER;
-#pragma unroll
-          for (int i = 0; i < PER; i += 2)
-            *reinterpret_cast<uint32_t*>(at + i) = pack_half2(acc[i] * inv, acc[i + 1] * inv);
-        }
-      }
-    }
-    u += last - first;
-    if (!more || next_w.tiles == 0) break;
     w = next_w;
 #pragma unroll
     for (int i = 0; i < 2; ++i) limit[i] = next_limit[i], dst[i] = next_dst[i];
@@ -610,19 +727,66 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
 
 int few_ctas(const adr_ctx* ctx) { return 2 * (ctx->sm_count > 0 ? ctx->sm_count : 148); }
 
+// Two slots to each of the chunks, ROWS rows to a slot.
 template <int HD, int WM>
-int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, const CUtensorMap& mv, const FewParams& p) {
+constexpr size_t few_rows(size_t ctas) {
+  using Cfg = FewCfg<HD, WM>;
+  return 2 * ctas * (1 + Cfg::SPARE) * Cfg::ROWS;
+}
+// The queue and the number of chunks, then their first segments.
+constexpr size_t FEW_HEAD = 256;
+size_t few_begins(size_t ctas) { return (3 * ctas * sizeof(Segment) + 255) / 256 * 256; }
+
+template <int HD, int WM>
+int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, const CUtensorMap& mv, FewParams p,
+                  double units) {
   using Cfg = FewCfg<HD, WM>;
   auto kfn = attention_few_kernel<HD, WM>;
   if (int rc = opt_in_smem(ctx, kfn, Cfg::SMEM); rc != ADR_OK) return rc;
-  return launch_whole_sm(ctx, stream, kfn, dim3(few_ctas(ctx)), FEW_THREADS, Cfg::SMEM, 1, true, mk, mv, p);
+  const int g = few_ctas(ctx);
+  p.spare = Cfg::SPARE;
+  p.part_ml = p.part_o + few_rows<HD, WM>(g) * HD;
+  const int ctas = (int)std::min<double>(g, units);
+  if (int rc = launch_whole_sm(ctx, stream, kfn, dim3(ctas), FEW_THREADS, Cfg::SMEM, 1, true, mk, mv, p); rc != ADR_OK)
+    return rc;
+  // the borders between the chunks: none where a CTA is all there is
+  const int borders = (int)std::min<double>(ctas * (1 + Cfg::SPARE), units) - 1;
+  if (borders < 1) return ADR_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(borders);
+  cfg.blockDim = dim3(JOIN_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, few_join_kernel<HD, Cfg::ROWS>, p);
+  if (e != cudaSuccess) {
+    ctx->last_cuda_error = (int)e;
+    return ADR_ERR_CUDA;
+  }
+  return after_launch(ctx);
+}
+
+// What the units of the launch can be at most: tiles of `rows` rows, blocks of the longest table row.
+double few_units(const SeqAttention& a, int rows, bool one_tile_each) {
+  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  const double tiles = one_tile_each ? a.n_seqs : (double)a.tokens * a.group / tile + a.n_seqs;
+  const double blocks = (double)(((long long)a.max_pages * a.page_size + FEW_KB - 1) / FEW_KB);
+  return tiles * blocks * a.n_kv_heads;
 }
 
 }  // namespace
 
 size_t attention_few_workspace(const adr_ctx* ctx, int head_dim) {
   const size_t g = few_ctas(ctx);
-  return (g * sizeof(unsigned) + 255) / 256 * 256 + 2 * g * FEW_MAX_ROWS * (head_dim + 2) * sizeof(float);
+  const size_t rows = std::max({few_rows<128, 1>(g), few_rows<128, 2>(g), few_rows<128, 4>(g)});
+  return FEW_HEAD + few_begins(g) + rows * (head_dim + 2) * sizeof(float);
+}
+
+bool attention_few_takes(const SeqAttention& a, int rows, bool one_tile_each) {
+  return few_units(a, rows, one_tile_each) < 2e9;
 }
 
 int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int rows, int max_rows, void* workspace) {
@@ -630,21 +794,23 @@ int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& 
   p.a = a;
   p.max_rows = max_rows;
   p.min_units = std::max(1, ctx->tune_att_cs.load());
+  p.spare_units = 16;
   p.page_rows = a.page_size < FEW_KB ? a.page_size : FEW_KB;
-  const size_t g = few_ctas(ctx);
-  p.counters = static_cast<unsigned int*>(workspace);
-  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (g * sizeof(unsigned) + 255) / 256 * 256);
-  p.part_o = p.part_ml + 2 * g * FEW_MAX_ROWS * 2;
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  p.queue = reinterpret_cast<unsigned int*>(at);
+  p.begins = reinterpret_cast<Segment*>(at + FEW_HEAD);
+  p.part_o = reinterpret_cast<float*>(at + FEW_HEAD + few_begins(few_ctas(ctx)));
   CUtensorMap mk, mv;
   if (int rc = pool_map(ctx, &mk, a.k, a.sk, a, p.page_rows); rc != ADR_OK) return rc;
   if (int rc = pool_map(ctx, &mv, a.v, a.sv, a, p.page_rows); rc != ADR_OK) return rc;
+  const double units = few_units(a, rows, max_rows <= 64);
   if (a.head_dim == 128)
-    return rows <= 16   ? launch_few_as<128, 1>(ctx, stream, mk, mv, p)
-           : rows <= 32 ? launch_few_as<128, 2>(ctx, stream, mk, mv, p)
-                        : launch_few_as<128, 4>(ctx, stream, mk, mv, p);
-  return rows <= 16   ? launch_few_as<64, 1>(ctx, stream, mk, mv, p)
-         : rows <= 32 ? launch_few_as<64, 2>(ctx, stream, mk, mv, p)
-                      : launch_few_as<64, 4>(ctx, stream, mk, mv, p);
+    return rows <= 16   ? launch_few_as<128, 1>(ctx, stream, mk, mv, p, units)
+           : rows <= 32 ? launch_few_as<128, 2>(ctx, stream, mk, mv, p, units)
+                        : launch_few_as<128, 4>(ctx, stream, mk, mv, p, units);
+  return rows <= 16   ? launch_few_as<64, 1>(ctx, stream, mk, mv, p, units)
+         : rows <= 32 ? launch_few_as<64, 2>(ctx, stream, mk, mv, p, units)
+                      : launch_few_as<64, 4>(ctx, stream, mk, mv, p, units);
 }
 
 }  // namespace adr

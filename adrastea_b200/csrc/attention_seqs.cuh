@@ -33,6 +33,8 @@ inline int pool_map(adr_ctx* ctx, CUtensorMap* map, const __half* base, const lo
 
 // Kernels of a few rows per sequence (attention_few.cu): `rows` rows of a key head at most chooses the tile,
 // sequences with more than max_rows are passed over.
+// attention_few_takes: whether its counts fit (`one_tile_each`: no sequence has more than `rows` rows).
+bool attention_few_takes(const SeqAttention& a, int rows, bool one_tile_each);
 size_t attention_few_workspace(const adr_ctx* ctx, int head_dim);
 int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int rows, int max_rows,
                          void* workspace);
