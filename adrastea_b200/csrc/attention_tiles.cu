@@ -26,6 +26,9 @@ namespace {
 
 constexpr int TL_M = 128;   // rows of a tile
 constexpr int TL_N = 128;   // keys of a block
+#ifndef TL_BY_FMA
+#define TL_BY_FMA 1
+#endif
 
 template <int HD, int NT>
 struct TileCfg {
@@ -35,7 +38,9 @@ struct TileCfg {
   static constexpr int THREADS = NT * 128 + 64;
   static constexpr uint32_t COLS = NT == 2 ? 512 : 256;
   static constexpr uint32_t O_COL = NT * 128;
-  static constexpr size_t SMEM = 1024 + (size_t)TILE * (NT + SLOTS) + 8 * (3 * NT + NT + 2 * SLOTS) + 64;
+  // of every eight pairs of probabilities, those that the FMA units compute (the others: the exponential unit)
+  static constexpr int BY_FMA = TL_BY_FMA;
+  static constexpr size_t SMEM = 1024 + (size_t)TILE * (NT + SLOTS) + 8 * (5 * NT + 2 * SLOTS) + 64;
 };
 
 struct TileParams {
@@ -68,6 +73,13 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t addr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_x16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_x8(uint32_t addr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -78,17 +90,117 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t addr, const uint32_t (&r)[8]
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// A from tensor memory
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The tensor-core warp runs its code with all lanes, so that addresses and descriptors are the same for all of them and
+// live in uniform registers; only the instructions themselves are one lane's.  (With one lane in a branch of its own
+// each of these instructions was preceded by moves of its six operands: 80 to 110 cycles where the tensor cores take 64.)
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
+  return r;
+}
+// Lower words of the descriptors of tcgen05.cuh; the upper word is the same for both kinds.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16); }
+template <bool ACC>
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred e, p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 e, %5, 0;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "n"(DESC_HI), "r"(idesc), "r"(leader), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+// A from tensor memory
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate,
+                                        uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t.reg .b64 b;\n\tsetp.ne.u32 e, %5, 0;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "n"(DESC_HI), "r"(idesc), "r"(leader), "r"(accumulate)
+      : "memory");
+}
+// mbar_wait in few instructions where the phase is complete, and with no call in it (a call would cost the caller its
+// uniform registers): the clock is looked at every 256th time only.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
+  long long t0 = 0;
+  for (uint32_t n = 0;; ++n) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+    if ((n & 255u) == 255u) {
+      const long long t = clock64();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > kWaitLimitCycles) return false;
+    }
+  }
+}
+__device__ __forceinline__ void arrive_bar(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit_one(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of both by the FMA units: x = n + f with n the nearest integer (the rounding of a sum with 1.5 * 2^23, whose low
+// bits are n), 2^f on [-1/2, 1/2] by the polynomial of degree 4 of least relative error (Remez exchange in 64 bits:
+// 2.6e-6, below the 2^-11 that the result is rounded to), times 2^n.  Below -126 the result is 2^-126, which is zero in
+// fp16; NaN stays NaN.
+__device__ __forceinline__ uint64_t exp2_fma2(uint64_t x2) {
+  float2 x = of_pair(x2);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
+  x2 = pair_of(x.x, x.y);
+  const uint64_t t = add2(x2, pair_of(12582912.0f, 12582912.0f));
+  const uint64_t n = add2(t, pair_of(-12582912.0f, -12582912.0f));
+  const uint64_t f = fma2(n, pair_of(-1.0f, -1.0f), x2);
+  uint64_t q = fma2(f, pair_of(0.009570102207f, 0.009570102207f), pair_of(0.055917859077f, 0.055917859077f));
+  q = fma2(f, q, pair_of(0.240247443318f, 0.240247443318f));
+  q = fma2(f, q, pair_of(0.693121790886f, 0.693121790886f));
+  q = fma2(f, q, pair_of(0.999999284744f, 0.999999284744f));
+  const float2 tf = of_pair(t);
+  return mul2(q, pair_of(__int_as_float((__float_as_int(tf.x) << 23) + 0x3F800000),
+                         __int_as_float((__float_as_int(tf.y) << 23) + 0x3F800000)));
 }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -123,7 +235,8 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + SLOTS * TILE);  // [NT]
   uint64_t* s_ready = q_full + NT;   // [NT] scores of a tile are complete
   uint64_t* p_ready = s_ready + NT;  // [NT] its probabilities are
-  uint64_t* o_done = p_ready + NT;   // [NT] its output is
+  uint64_t* p_half = p_ready + NT;   // [NT] those of the first 64 keys are
+  uint64_t* o_done = p_half + NT;    // [NT] its output is
   uint64_t* full = o_done + NT;      // [SLOTS]
   uint64_t* empty = full + SLOTS;    // [SLOTS]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + SLOTS);
@@ -140,6 +253,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       mbar_init(&q_full[i], 1);
       mbar_init(&s_ready[i], 1);
       mbar_init(&p_ready[i], 4);
+      mbar_init(&p_half[i], 4);
       mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < SLOTS; ++i) {
@@ -263,58 +377,91 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     if (!ok && lane == 0) atomicOr(p.a.status, 1u << 23);
   } else if (warp == W_MMA) {
     // ------------------------------- tensor cores -------------------------------
-    if (lane == 0 && nb_max > 0) {
+    if (nb_max > 0) {
+      // (Nothing here leaves the loops early: a lane whose wait ran out skips the waits and instructions that follow.)
       bool ok = true;
+      const uint32_t leader = elect_one();
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_lo = desc_lo(smem_u32(q_sm), 16), k_lo = desc_lo(smem_u32(ring), 16),
+                     v_lo = desc_lo(smem_u32(ring), TL_N * 128);
+      const uint32_t b_q = smem_u32(q_full), b_s = smem_u32(s_ready), b_p = smem_u32(p_ready), b_h = smem_u32(p_half),
+                     b_o = smem_u32(o_done), b_full = smem_u32(full), b_empty = smem_u32(empty);
+      constexpr uint32_t CHUNK = TL_N * 128 / 16, SLOT = TILE / 16;  // steps of a descriptor
+      int all_see[NT];  // keys that every row of a tile sees
+#pragma unroll
+      for (int t = 0; t < NT; ++t) all_see[t] = p.a.causal ? max(0, lk - lq + token0 + t * p.tokens_tile + 1) : lk;
       uint32_t have_o[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) have_o[t] = 0;
-      auto wait_full = [&](int i) { ok = ok && mbar_wait(&full[i % SLOTS], (unsigned)(i / SLOTS) & 1u); };
-      // the last tile that uses block j (tile 1 sees at least what tile 0 sees)
-      auto last_of = [&](int j) { return NT == 2 && j < nb[NT - 1] ? 1 : 0; };
-      auto scores = [&](int t, int j) {
-        if (j == 0) ok = ok && mbar_wait(&q_full[t], 0);
-        wait_full(2 * j);
-        if (!ok) return;
+      // (the vote tells the compiler, too, that the lanes are together again)
+      auto wait = [&](uint32_t bar, uint32_t parity) { ok = __all_sync(0xffffffffu, ok && wait_bar(bar, parity)); };
+      auto k_slot = [](int j) { return (uint32_t)(2 * j) % SLOTS; };
+      auto v_slot = [](int j) { return (uint32_t)(2 * j + 1) % SLOTS; };
+      auto wait_k = [&](int j) { wait(b_full + k_slot(j) * 8, ((uint32_t)(2 * j) / SLOTS) & 1u); };
+      auto wait_v = [&](int j) { wait(b_full + v_slot(j) * 8, ((uint32_t)(2 * j + 1) / SLOTS) & 1u); };
+      auto scores = [&](int t, int j, bool last) {
         tc_fence_after_sync();
-        const uint32_t idesc = umma_idesc_f16(block_n(t, j), false);
-        const uint32_t qa = smem_u32(q_sm + t * TILE), ka = smem_u32(ring + ((2 * j) % SLOTS) * TILE);
+        if (!ok) return;
+        const uint32_t idesc = umma_idesc_f16(block_n(t, j), false), go = leader;
+        const uint32_t qa = q_lo + t * SLOT, ka = k_lo + k_slot(j) * SLOT;
+        umma_ss<false>(tm + t * 128, qa, ka, idesc, go);
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f16(tmem + t * 128, umma_desc_k_sw128(qa + c * (TL_M * 128)) + (uint64_t)(kk * 2),
-                     umma_desc_k_sw128(ka + c * (TL_N * 128)) + (uint64_t)(kk * 2), idesc, (c | kk) ? 1u : 0u);
-        umma_commit(&s_ready[t]);
-        if (t == last_of(j)) umma_commit(&empty[(2 * j) % SLOTS]);
+        for (int i = 1; i < CH * 4; ++i)
+          umma_ss<true>(tm + t * 128, qa + (i / 4) * CHUNK + (i % 4) * 2, ka + (i / 4) * CHUNK + (i % 4) * 2, idesc, go);
+        commit_one(b_s + t * 8, go);
+        if (last) commit_one(b_empty + k_slot(j) * 8, go);
       };
-      auto output = [&](int t, int j) {
-        ok = ok && mbar_wait(&p_ready[t], (unsigned)j & 1u);
-        wait_full(2 * j + 1);
-        if (!ok) return;
+      auto output = [&](int t, int j, bool last) {
+        wait(b_h + t * 8, (uint32_t)j & 1u);
         tc_fence_after_sync();
-        if (by_hand[t] == 0) {
-          constexpr uint32_t idesc = umma_idesc_f16(HD, true);
-          const uint64_t vd = umma_desc_mn_sw128(smem_u32(ring + ((2 * j + 1) % SLOTS) * TILE), TL_N * 128);
-          const int steps = block_n(t, j) / 16;
-          for (int ks = 0; ks < steps; ++ks)
-            umma_ts(tmem + Cfg::O_COL + t * HD, tmem + t * 128 + ks * 8, vd + (uint64_t)ks * 128, idesc,
-                    (have_o[t] | (uint32_t)ks) ? 1u : 0u);
+        constexpr uint32_t idesc = umma_idesc_f16(HD, true);
+        const uint32_t vd = v_lo + v_slot(j) * SLOT, d = tm + Cfg::O_COL + t * HD, a = tm + t * 128;
+        if ((j + 1) * TL_N <= all_see[t]) {
+          if (!ok) return;
+          const uint32_t go = leader;
+          umma_ts(d, a, vd, idesc, have_o[t], go);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) umma_ts(d, a + i * 8, vd + i * 128, idesc, 1u, go);
+          wait(b_p + t * 8, (uint32_t)j & 1u);
+          tc_fence_after_sync();
+          if (!ok) return;
+          const uint32_t go2 = leader;
+#pragma unroll
+          for (int i = 4; i < 8; ++i) umma_ts(d, a + i * 8, vd + i * 128, idesc, 1u, go2);
+        } else {
+          // a block that not every row sees whole: it may be short, or done already
+          wait(b_p + t * 8, (uint32_t)j & 1u);
+          tc_fence_after_sync();
+          if (!ok) return;
+          const uint32_t go = __shfl_sync(0xffffffffu, by_hand[t], 0) == 0 ? leader : 0;
+          const int n = block_n(t, j) / 16;
+          for (int i = 0; i < n; ++i) umma_ts(d, a + i * 8, vd + i * 128, idesc, have_o[t] | (uint32_t)i, go);
         }
         have_o[t] = 1;
-        if (t == last_of(j)) umma_commit(&empty[(2 * j + 1) % SLOTS]);
-        if (j == nb[t] - 1) umma_commit(&o_done[t]);
+        const uint32_t go = leader;
+        if (last) commit_one(b_empty + v_slot(j) * 8, go);
+        if (j == nb[t] - 1) commit_one(b_o + t * 8, go);
       };
+      // tile 1 sees at least what tile 0 sees, so a block's last user is tile 1 where it takes part
+      auto last = [&](int t, int j) { return NT == 1 || t == 1 || j >= nb[NT - 1]; };
+      wait_k(0);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        if (nb[t] > 0) scores(t, 0);
+      for (int t = 0; t < NT; ++t) {
+        if (nb[t] == 0) continue;
+        wait(b_q + t * 8, 0);
+        scores(t, 0, last(t, 0));
+      }
+#pragma unroll 1
       for (int j = 0; j < nb_max && ok; ++j) {
+        wait_v(j);
+        if (j + 1 < nb_max) wait_k(j + 1);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          if (j < nb[t]) output(t, j);
-          if (j + 1 < nb[t]) scores(t, j + 1);
+          if (j < nb[t]) output(t, j, last(t, j));
+          if (j + 1 < nb[t]) scores(t, j + 1, last(t, j + 1));
         }
       }
-      if (!ok) atomicOr(p.a.status, 1u << 24);
+      if (!ok && lane == 0) atomicOr(p.a.status, 1u << 24);
     }
   } else {
     // ------------------------------- softmax and output -------------------------------
@@ -338,30 +485,45 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
 
+    const uint32_t b_s = smem_u32(&s_ready[t]), b_p = smem_u32(&p_ready[t]), b_h = smem_u32(&p_half[t]);
     for (int j = 0; j < my_nb; ++j) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_ready[t], (unsigned)j & 1u));
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_s, (unsigned)j & 1u));
       tc_fence_after_sync();
       const int key0 = j * TL_N;
       const bool partly = key0 + TL_N > all_see;  // some row does not see some key of the block
       bool hand = false;
       if (ok && warp_live) {
-        uint32_t s[128];
+        if (partly || negative) {
+          // the scores as they are to be, written back over the others
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            uint32_t s[32];
+            tmem_ld_x32(s_at + c, s);
+            tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_x32(s_at + c * 32, s + c * 32);
-        tmem_ld_wait();
-        if (negative) {
-#pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] ^= 0x80000000u;
+            for (int i = 0; i < 32; ++i) {
+              if (negative) s[i] ^= 0x80000000u;
+              if (key0 + c + i >= limit) s[i] = 0xFF800000u;  // -infinity
+            }
+            tmem_st_x32(s_at + c, s);
+          }
+          tmem_wait_st();
         }
-        if (partly) {
+        // the row's maximum
+        float mx;
+        {
+          uint32_t s[128];
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (key0 + i >= limit) s[i] = 0xFF800000u;  // -infinity
+          for (int c = 0; c < 4; ++c) tmem_ld_x32(s_at + c * 32, s + c * 32);
+          tmem_ld_wait();
+          float top[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+#pragma unroll
+          for (int i = 16; i < 128; i += 2)
+            top[(i >> 1) & 7] = max3(top[(i >> 1) & 7], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          mx = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), fmaxf(top[6], top[7]));
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         // (a first maximum moves from -infinity: nothing is summed or in O yet but zeros)
         const bool move = mx > m + slack || (m == -INFINITY && mx > m);
         if (__any_sync(0xffffffffu, move)) {
@@ -381,20 +543,44 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
           }
         }
         const float base = m == -INFINITY ? 0.0f : m * scale2;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t mul = pair_of(scale2, scale2), sub = pair_of(-base, -base);
+        uint64_t sum[2] = {0, 0};
+        // The scores are read a second time, 32 at a time and 32 ahead, rather than kept: that leaves registers for many
+        // exponentials at once.  Probabilities are written over scores that have been read.
+        uint32_t s[2][32];
+        tmem_ld_x32(s_at, s[0]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[32];
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait();
+          if (c < 3) tmem_ld_x32(s_at + (c + 1) * 32, s[(c + 1) & 1]);
+          uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float a = exp2_fast(fmaf(__uint_as_float(s[c * 64 + 2 * i]), scale2, -base));
-            const float b = exp2_fast(fmaf(__uint_as_float(s[c * 64 + 2 * i + 1]), scale2, -base));
-            sum[i & 3] += a + b;
-            pk[i] = pack_half2(a, b);
+          for (int i = 0; i < 16; ++i) {
+            uint64_t x = fma2(pair_of(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), mul, sub);
+            if ((i & 7) >= 8 - Cfg::BY_FMA) {
+              x = exp2_fma2(x);
+            } else {
+              const float2 e = of_pair(x);
+              x = pair_of(exp2_fast(e.x), exp2_fast(e.y));
+            }
+            sum[i & 1] = add2(sum[i & 1], x);
+            const float2 e = of_pair(x);
+            pk[i] = pack_half2(e.x, e.y);
           }
-          tmem_st_x32(s_at + c * 32, pk);
+          tmem_st_x16(s_at + c * 16, pk);
+          if (c == 1) {
+            // the tensor cores may begin
+            tmem_wait_st();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive_bar(b_h);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float2 total = of_pair(add2(sum[0], sum[1]));
+        l += total.x + total.y;
+      } else {
+        __syncwarp();
+        if (lane == 0) arrive_bar(b_h);
       }
       tmem_wait_st();
       if (partly) {
@@ -455,10 +641,10 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
           tmem_wait_st();
         }
       }
-      if (row == 0) by_hand[t] = hand ? 1u : 0u;
+      if (partly && row == 0) by_hand[t] = hand ? 1u : 0u;
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t]);
+      if (lane == 0) arrive_bar(b_p);
     }
     if (my_nb > 0) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], 0));

@@ -46,7 +46,7 @@ def attend(q, k, v, scale, first):
 
     Bound, per element: a probability is rounded to fp16 (2^-11 of it, 2^-25 where it is subnormal, against a sum of at
     least sum exp(s - max)) and its score, a sum of hd products in fp32, is off by hd * 2^-23 of the sum of their sizes,
-    and by 2^-22 of its distance from the maximum in the exponential; exp itself by 2^-21; the output's rounding is 2^-11
+    and by 2^-22 of its distance from the maximum in the exponential; exp itself by 2^-18 (a polynomial of degree 4); the output's rounding is 2^-11
     of it.  fp32 sums over the keys add sqrt-like 2^-24s, covered by the factor 1.05."""
     m, H, hd = q.shape
     n, Hk = k.shape[:2]
@@ -70,7 +70,7 @@ def attend(q, k, v, scale, first):
         l = torch.where(some[:, None], l, torch.ones_like(l))
         vh_ = torch.where(seen.any(0)[:, None], vh, torch.zeros_like(vh))  # what nobody sees does not count
         o = (e / l) @ vh_
-        off = 2.0 ** -11 + 2 * (hd * 2.0 ** -23) * size + 2.0 ** -22 * (s - top).masked_fill(~seen, 0).abs() * 2 + 2.0 ** -20
+        off = 2.0 ** -11 + 2 * (hd * 2.0 ** -23) * size + 2.0 ** -22 * (s - top).masked_fill(~seen, 0).abs() * 2 + 2.0 ** -18
         t = (e / l * off) @ vh_.abs() + 2.0 ** -25 * (seen.double() @ vh_.abs()) / l
         out[:, h] = torch.where(some[:, None], o, torch.zeros_like(o))
         tol[:, h] = torch.where(some[:, None], 1.05 * t + o.abs() * 2.0 ** -11 + 2.0 ** -25, torch.zeros_like(t))
