@@ -26,9 +26,8 @@ namespace {
 
 constexpr int TL_M = 128;   // rows of a tile
 constexpr int TL_N = 128;   // keys of a block
-#ifndef TL_BY_FMA
-#define TL_BY_FMA 1
-#endif
+// Of every eight pairs of probabilities, those that the FMA units compute; the others go to the exponential unit.
+constexpr int BY_FMA = 1;
 
 template <int HD, int NT>
 struct TileCfg {
@@ -38,8 +37,7 @@ struct TileCfg {
   static constexpr int THREADS = NT * 128 + 64;
   static constexpr uint32_t COLS = NT == 2 ? 512 : 256;
   static constexpr uint32_t O_COL = NT * 128;
-  // of every eight pairs of probabilities, those that the FMA units compute (the others: the exponential unit)
-  static constexpr int BY_FMA = TL_BY_FMA;
+
   static constexpr size_t SMEM = 1024 + (size_t)TILE * (NT + SLOTS) + 8 * (5 * NT + 2 * SLOTS) + 64;
 };
 
@@ -475,6 +473,8 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     const bool warp_live = __any_sync(0xffffffffu, live);
     const int limit = !live ? 0 : p.a.causal ? max(0, lk - lq + first + tok + 1) : lk;
     const int all_see = p.a.causal ? max(0, lk - lq + first + 1) : lk;  // keys that every row of the tile sees
+    const int warp_most = __reduce_max_sync(0xffffffffu, limit);  // keys that some row of the warp sees
+    const int my_end = NT == 2 && t == 1 ? kend[NT - 1] : kend[0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + (uint32_t)(t * 128), o_at = tmem + lanes + Cfg::O_COL + (uint32_t)(t * HD);
     // scores in powers of two; the sign of the scale goes into the scores so that the largest product is the maximum
@@ -487,31 +487,46 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
 
     const uint32_t b_s = smem_u32(&s_ready[t]), b_p = smem_u32(&p_ready[t]), b_h = smem_u32(&p_half[t]);
     for (int j = 0; j < my_nb; ++j) {
-      if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_s, (unsigned)j & 1u));
-      tc_fence_after_sync();
       const int key0 = j * TL_N;
       const bool partly = key0 + TL_N > all_see;  // some row does not see some key of the block
+      uint8_t* v = ring + ((2 * j + 1) % SLOTS) * TILE;
       bool hand = false;
-      if (ok && warp_live) {
-        if (partly || negative) {
-          // the scores as they are to be, written back over the others
-#pragma unroll 1
-          for (int c = 0; c < 128; c += 32) {
-            uint32_t s[32];
-            tmem_ld_x32(s_at + c, s);
-            tmem_ld_wait();
+      if (partly) {
+        // While the scores are computed: V is waited for, cleared behind the end, and searched for what may not be
+        // multiplied by zero.  A thread takes a 16-byte piece of every 128 / (HD / 8)-th row (the swizzle only permutes
+        // a row's pieces).
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[(2 * j + 1) % SLOTS], (unsigned)((2 * j + 1) / SLOTS) & 1u));
+        const int from = max(0, all_see - key0), end = min(TL_N, lk - key0);
+        constexpr int LPR = HD / 8, STEP = 128 / LPR;
+        uint4* at = reinterpret_cast<uint4*>(v + ((row % LPR) / 8) * (TL_N * 128) + (row % 8) * 16);
+        uint32_t odd = 0;
+        int r = from + row / LPR;
+        for (; r + 3 * STEP < end; r += 4 * STEP) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (negative) s[i] ^= 0x80000000u;
-              if (key0 + c + i >= limit) s[i] = 0xFF800000u;  // -infinity
-            }
-            tmem_st_x32(s_at + c, s);
+          for (int i = 0; i < 4; ++i) {
+            const uint4 x = at[(r + i * STEP) * 8];
+            odd |= not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w);
           }
-          tmem_wait_st();
         }
+#pragma unroll 1
+        for (; r < TL_N; r += STEP) {
+          if (r >= end) {
+            at[r * 8] = make_uint4(0, 0, 0, 0);
+          } else {
+            const uint4 x = at[r * 8];
+            odd |= not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w);
+          }
+        }
+        fence_proxy_async();
+        hand = tile_any(t, odd != 0);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_s, (unsigned)j & 1u));
+      tc_fence_after_sync();
+      if (ok && warp_live) {
+        const int chunks = partly ? (min(TL_N, my_end - key0) + 31) / 32 : 4;  // of 32 keys
         // the row's maximum
         float mx;
-        {
+        if (!partly && !negative) {
           uint32_t s[128];
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld_x32(s_at + c * 32, s + c * 32);
@@ -523,6 +538,25 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
           for (int i = 16; i < 128; i += 2)
             top[(i >> 1) & 7] = max3(top[(i >> 1) & 7], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
           mx = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), fmaxf(top[6], top[7]));
+        } else {
+          // the scores as they are to be, written back; what no row of the warp sees is passed over
+          mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < chunks; ++c) {
+            const int k = key0 + c * 32;
+            if (k >= warp_most) break;
+            uint32_t s[32];
+            tmem_ld_x32(s_at + c * 32, s);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (negative) s[i] ^= 0x80000000u;
+              if (k + i >= limit) s[i] = 0xFF800000u;  // -infinity
+              mx = fmaxf(mx, __uint_as_float(s[i]));
+            }
+            tmem_st_x32(s_at + c * 32, s);
+          }
+          tmem_wait_st();
         }
         // (a first maximum moves from -infinity: nothing is summed or in O yet but zeros)
         const bool move = mx > m + slack || (m == -INFINITY && mx > m);
@@ -545,19 +579,11 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         const float base = m == -INFINITY ? 0.0f : m * scale2;
         const uint64_t mul = pair_of(scale2, scale2), sub = pair_of(-base, -base);
         uint64_t sum[2] = {0, 0};
-        // The scores are read a second time, 32 at a time and 32 ahead, rather than kept: that leaves registers for many
-        // exponentials at once.  Probabilities are written over scores that have been read.
-        uint32_t s[2][32];
-        tmem_ld_x32(s_at, s[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait();
-          if (c < 3) tmem_ld_x32(s_at + (c + 1) * 32, s[(c + 1) & 1]);
-          uint32_t pk[16];
+        auto powers = [&](const uint32_t (&s)[32], uint32_t (&pk)[16]) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            uint64_t x = fma2(pair_of(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), mul, sub);
-            if ((i & 7) >= 8 - Cfg::BY_FMA) {
+            uint64_t x = fma2(pair_of(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), mul, sub);
+            if ((i & 7) >= 8 - BY_FMA) {
               x = exp2_fma2(x);
             } else {
               const float2 e = of_pair(x);
@@ -567,84 +593,93 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
             const float2 e = of_pair(x);
             pk[i] = pack_half2(e.x, e.y);
           }
-          tmem_st_x16(s_at + c * 16, pk);
-          if (c == 1) {
-            // the tensor cores may begin
-            tmem_wait_st();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive_bar(b_h);
+        };
+        // The scores are read a second time, 32 at a time and 32 ahead, rather than kept: that leaves registers for many
+        // exponentials at once.  Probabilities are written over scores that have been read.
+        if (!partly) {
+          uint32_t s[2][32];
+          tmem_ld_x32(s_at, s[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            if (c < 3) tmem_ld_x32(s_at + (c + 1) * 32, s[(c + 1) & 1]);
+            uint32_t pk[16];
+            powers(s[c & 1], pk);
+            tmem_st_x16(s_at + c * 16, pk);
+            if (c == 1) {
+              // the tensor cores may begin
+              tmem_wait_st();
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) arrive_bar(b_h);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < chunks; ++c) {
+            uint32_t pk[16];
+            if (key0 + c * 32 < warp_most) {
+              uint32_t s[32];
+              tmem_ld_x32(s_at + c * 32, s);
+              tmem_ld_wait();
+              powers(s, pk);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0;
+            }
+            tmem_st_x16(s_at + c * 16, pk);
           }
         }
         const float2 total = of_pair(add2(sum[0], sum[1]));
         l += total.x + total.y;
-      } else {
-        __syncwarp();
-        if (lane == 0) arrive_bar(b_h);
       }
       tmem_wait_st();
-      if (partly) {
-        // V: wait for it, clear what lies behind the end, look for what may not be multiplied by zero
-        uint8_t* v = ring + ((2 * j + 1) % SLOTS) * TILE;
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[(2 * j + 1) % SLOTS], (unsigned)((2 * j + 1) / SLOTS) & 1u));
-        const int from = max(0, all_see - key0), end = min(TL_N, lk - key0);
-        uint32_t odd = 0;
-        // a thread takes a 16-byte piece of every 128 / (HD / 8)-th row (the swizzle only permutes a row's pieces)
-        constexpr int LPR = HD / 8;
-        for (int r = from + row / LPR; r < TL_N; r += 128 / LPR) {
-          uint4* at = reinterpret_cast<uint4*>(v + ((row % LPR) / 8) * (TL_N * 128) + r * 128 + (row % 8) * 16);
-          if (r >= end) {
-            *at = make_uint4(0, 0, 0, 0);
-          } else {
-            const uint4 x = *at;
-            odd |= not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w);
+      if (hand && ok && warp_live) {
+        // this block's product by hand
+        const int end = min(TL_N, my_end - key0);
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 8) {
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = 0;
+          if (j > 0) {
+            tmem_ld_x8(o_at + c, o);
+            tmem_ld_wait();
           }
-        }
-        fence_proxy_async();
-        hand = tile_any(t, odd != 0);
-        if (hand && ok && warp_live) {
-          // this block's product by hand
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 8) {
-            uint32_t o[8];
+          for (int k0 = 0; k0 < end; k0 += 16) {
+            uint32_t pk[8];
+            __syncwarp();
+            tmem_ld_x8(s_at + k0 / 2, pk);
+            tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = 0;
-            if (j > 0) {
-              tmem_ld_x8(o_at + c, o);
-              tmem_ld_wait();
-            }
-#pragma unroll 1
-            for (int k0 = 0; k0 < end; k0 += 16) {
-              uint32_t pk[8];
-              __syncwarp();
-              tmem_ld_x8(s_at + k0 / 2, pk);
-              tmem_ld_wait();
+            for (int k = 0; k < 16; ++k) {
+              const __half2 ph = *reinterpret_cast<const __half2*>(&pk[k >> 1]);
+              const float w = (k & 1) ? __high2float(ph) : __low2float(ph);
+              const int r = k0 + k;
+              if (key0 + r >= limit) continue;  // (also what lies behind the end)
+              const uint4 x = *reinterpret_cast<const uint4*>(v + (c / 64) * (TL_N * 128) + r * 128 + (((c / 8) ^ r) & 7) * 16);
+              const __half2* h = reinterpret_cast<const __half2*>(&x);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const __half2 ph = *reinterpret_cast<const __half2*>(&pk[k >> 1]);
-                const float w = (k & 1) ? __high2float(ph) : __low2float(ph);
-                const int r = k0 + k;
-                if (key0 + r >= limit) continue;  // (also what lies behind the end)
-                const uint4 x = *reinterpret_cast<const uint4*>(v + (c / 64) * (TL_N * 128) + r * 128 + (((c / 8) ^ r) & 7) * 16);
-                const __half2* h = reinterpret_cast<const __half2*>(&x);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 f = __half22float2(h[i]);
-                  o[2 * i] = __float_as_uint(fmaf(w, f.x, __uint_as_float(o[2 * i])));
-                  o[2 * i + 1] = __float_as_uint(fmaf(w, f.y, __uint_as_float(o[2 * i + 1])));
-                }
+              for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(h[i]);
+                o[2 * i] = __float_as_uint(fmaf(w, f.x, __uint_as_float(o[2 * i])));
+                o[2 * i + 1] = __float_as_uint(fmaf(w, f.y, __uint_as_float(o[2 * i + 1])));
               }
             }
-            __syncwarp();
-            tmem_st_x8(o_at + c, o);
           }
-          tmem_wait_st();
+          __syncwarp();
+          tmem_st_x8(o_at + c, o);
         }
+        tmem_wait_st();
       }
       if (partly && row == 0) by_hand[t] = hand ? 1u : 0u;
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) arrive_bar(b_p);
+      if (lane == 0) {
+        if (partly || !ok || !warp_live) arrive_bar(b_h);
+        arrive_bar(b_p);
+      }
     }
     if (my_nb > 0) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], 0));
