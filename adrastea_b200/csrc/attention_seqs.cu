@@ -73,12 +73,12 @@ extern "C" int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, 
   }
   p.scale = scale;
   p.status = ctx->d_status;
-  return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1);
+  return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1, nullptr);
 }
 
 extern "C" size_t adr_attention_paged_workspace(const adr_ctx* ctx, int n_heads, int n_kv_heads, int head_dim) {
   if (!ctx || check_heads(n_heads, n_kv_heads, head_dim) != ADR_OK) return 0;
-  return attention_few_workspace(ctx, head_dim);
+  return std::max(attention_few_workspace(ctx, head_dim), attention_tiles_workspace(ctx, head_dim));
 }
 
 extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, const void* q, const void* k_pages,
@@ -135,7 +135,9 @@ extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, c
   const long long rows = (long long)max_q * p.group;
   if (rows <= FEW_ROWS && attention_few_takes(p, (int)rows, false)) return launch_attention_few(ctx, (cudaStream_t)stream, p, (int)rows, INT_MAX, workspace);
   // all sequences of one length: tiles for all; otherwise those of few rows go to the other kernel
-  if ((long long)n_seqs * max_q == tokens || !attention_few_takes(p, FEW_ROWS, true)) return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1);
-  if (int rc = launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, FEW_ROWS + 1); rc != ADR_OK) return rc;
+  if ((long long)n_seqs * max_q == tokens || !attention_few_takes(p, FEW_ROWS, true))
+    return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1, workspace);
+  if (int rc = launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, FEW_ROWS + 1, workspace); rc != ADR_OK)
+    return rc;
   return launch_attention_few(ctx, (cudaStream_t)stream, p, FEW_ROWS, FEW_ROWS, workspace);
 }

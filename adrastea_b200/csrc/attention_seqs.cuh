@@ -39,8 +39,10 @@ size_t attention_few_workspace(const adr_ctx* ctx, int head_dim);
 int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int rows, int max_rows,
                          void* workspace);
 
-// Tiles of many rows (attention_tiles.cu): `max_q` chooses the tiles of a CTA, sequences with fewer than min_rows rows
-// of a key head are passed over.
-int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int max_q, int min_rows);
+// Tiles of many rows (attention_tiles.cu): sequences with fewer than min_rows rows of a key head are passed over.  The
+// workspace is used over pages only.
+size_t attention_tiles_workspace(const adr_ctx* ctx, int head_dim);
+int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int max_q, int min_rows,
+                           void* workspace);
 
 }  // namespace adr

@@ -26,6 +26,8 @@ namespace {
 
 constexpr int TL_M = 128;   // rows of a tile
 constexpr int TL_N = 128;   // keys of a block
+// The workspace: the first bytes are the other kernel's queue, which has to stay as it is.
+constexpr size_t TL_JOBS_AT = 256, TL_PARTS_AT = 16384;
 // Of every eight pairs of probabilities, those that the FMA units compute; the others go to the exponential unit.
 constexpr int BY_FMA = 1;
 
@@ -33,7 +35,7 @@ template <int HD, int NT>
 struct TileCfg {
   static constexpr int CH = HD / 64;
   static constexpr int TILE = 128 * HD * 2;
-  static constexpr int SLOTS = NT == 2 ? (HD == 128 ? 5 : 8) : (HD == 128 ? 2 : 4);
+  static constexpr int SLOTS = NT == 2 ? 5 : (HD == 128 ? 2 : 4);
   static constexpr int THREADS = NT * 128 + 64;
   static constexpr uint32_t COLS = NT == 2 ? 512 : 256;
   static constexpr uint32_t O_COL = NT * 128;
@@ -41,11 +43,20 @@ struct TileCfg {
   static constexpr size_t SMEM = 1024 + (size_t)TILE * (NT + SLOTS) + 8 * (5 * NT + 2 * SLOTS) + 64;
 };
 
+struct TileJob {
+  SeqSpan span;
+  int s, token0;  // first token of the CTA's tiles; s past the last sequence: nothing to do
+};
+
 struct TileParams {
   SeqAttention a;
   int tokens_tile;   // tokens of a tile: 128 / group
   int min_rows;      // sequences with fewer rows of a key head than this are left to another kernel
   int page_rows;     // rows of a copy of keys: a page, 128 at most
+  int splits;        // parts of a job's keys, each for a CTA of its own
+  float2* part_ml;   // [jobs * splits][128]
+  float* part_o;     // [jobs * splits][128][head_dim]
+  TileJob* job_of;   // [jobs]
 };
 
 __device__ __forceinline__ void tmem_ld_x32(uint32_t addr, uint32_t* r) {
@@ -216,12 +227,7 @@ __device__ __forceinline__ bool tile_any(int tile, bool x) {
   return r != 0;
 }
 
-struct TileJob {
-  SeqSpan span;
-  int s, token0;  // first token of the CTA's tiles
-};
-
-template <int HD, int NT, bool PAGED>
+template <int HD, int NT, bool PAGED, bool SPLIT>
 __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TileParams p) {
@@ -266,10 +272,11 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
   tc_fence_after_sync();
   // (only now: a launch behind this one may not take the tensor memory that this CTA is waiting for)
   pdl_wait_trigger();
-  const int head = blockIdx.x % p.a.n_kv_heads;
+  const int job_id = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
+  const int head = job_id % p.a.n_kv_heads;
   if (warp == 0) {
     // the CTA's tiles: the last ones of a sequence, which see most keys, come first
-    int id = blockIdx.x / p.a.n_kv_heads;
+    int id = job_id / p.a.n_kv_heads;
     const int per = NT * p.tokens_tile;
     TileJob job = {};
     job.s = p.a.n_seqs;
@@ -296,7 +303,10 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       }
       id -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) s_job = job;
+    if (lane == 0) {
+      s_job = job;
+      if (SPLIT && blockIdx.x % p.splits == 0) p.job_of[job_id] = job;
+    }
   }
   __syncthreads();
   const uint32_t tmem = *tmem_slot;
@@ -313,8 +323,14 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     nb[t] = (kend[t] + TL_N - 1) / TL_N;
     nb_max = max(nb_max, nb[t]);
   }
+  int j0 = 0;  // this CTA's first block; blocks are counted from it
+  if constexpr (SPLIT) {
+    const int part = blockIdx.x % p.splits, all = nb[0];
+    j0 = all * part / p.splits;
+    nb[0] = nb_max = all * (part + 1) / p.splits - j0;
+  }
   // keys of a block as the tensor cores take them, in steps of 16
-  auto block_n = [&](int t, int j) { return min(TL_N, (kend[t] - j * TL_N + 15) & ~15); };
+  auto block_n = [&](int t, int j) { return min(TL_N, (kend[t] - (j0 + j) * TL_N + 15) & ~15); };
 
   if (warp == W_TMA) {
     // ------------------------------- producer -------------------------------
@@ -331,7 +347,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       }
       int issued = 0;
       for (int i = 0; i < 2 * nb_max; ++i) {
-        const int st = i % SLOTS, j = i >> 1;
+        const int st = i % SLOTS, j = j0 + (i >> 1);
         uint8_t* dst = ring + st * TILE;
         const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
         if constexpr (PAGED) {
@@ -414,7 +430,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         tc_fence_after_sync();
         constexpr uint32_t idesc = umma_idesc_f16(HD, true);
         const uint32_t vd = v_lo + v_slot(j) * SLOT, d = tm + Cfg::O_COL + t * HD, a = tm + t * 128;
-        if ((j + 1) * TL_N <= all_see[t]) {
+        if ((j0 + j + 1) * TL_N <= all_see[t]) {
           if (!ok) return;
           const uint32_t go = leader;
           umma_ts(d, a, vd, idesc, have_o[t], go);
@@ -487,14 +503,13 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
 
     const uint32_t b_s = smem_u32(&s_ready[t]), b_p = smem_u32(&p_ready[t]), b_h = smem_u32(&p_half[t]);
     for (int j = 0; j < my_nb; ++j) {
-      const int key0 = j * TL_N;
+      const int key0 = (j0 + j) * TL_N;
       const bool partly = key0 + TL_N > all_see;  // some row does not see some key of the block
       uint8_t* v = ring + ((2 * j + 1) % SLOTS) * TILE;
       bool hand = false;
-      if (partly) {
-        // While the scores are computed: V is waited for, cleared behind the end, and searched for what may not be
-        // multiplied by zero.  A thread takes a 16-byte piece of every 128 / (HD / 8)-th row (the swizzle only permutes
-        // a row's pieces).
+      // V is waited for, cleared behind the end, and searched for what may not be multiplied by zero.  A thread takes a
+      // 16-byte piece of every 128 / (HD / 8)-th row (the swizzle only permutes a row's pieces).
+      auto look_at_values = [&] {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[(2 * j + 1) % SLOTS], (unsigned)((2 * j + 1) / SLOTS) & 1u));
         const int from = max(0, all_see - key0), end = min(TL_N, lk - key0);
         constexpr int LPR = HD / 8, STEP = 128 / LPR;
@@ -519,9 +534,14 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         }
         fence_proxy_async();
         hand = tile_any(t, odd != 0);
-      }
+      };
+      // While the scores are computed; but a barrier's phase may be waited for only when the one before it is known to be
+      // complete, and with two slots that one is the V before, whose product the scores come behind.
+      const bool early = SLOTS > 2 || j == 0;
+      if (partly && early) look_at_values();
       if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_s, (unsigned)j & 1u));
       tc_fence_after_sync();
+      if (partly && !early) look_at_values();
       if (ok && warp_live) {
         const int chunks = partly ? (min(TL_N, my_end - key0) + 31) / 32 : 4;  // of 32 keys
         // the row's maximum
@@ -685,6 +705,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], 0));
       tc_fence_after_sync();
     }
+    if (SPLIT && ok && live) p.part_ml[(size_t)blockIdx.x * TL_M + row] = make_float2(m * scale2, l);
     if (ok && warp_live) {
       // a row that sees no key gets zeros
       const float inv = limit > 0 ? 1.0f / l : 0.0f;
@@ -697,7 +718,14 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
           tmem_ld_x32(o_at + c, o);
           tmem_ld_wait();
         }
-        if (live) {
+        if (SPLIT && live && my_nb > 0) {
+          float4* to = reinterpret_cast<float4*>(p.part_o + ((size_t)blockIdx.x * TL_M + row) * HD + c);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            __stcg(to + i / 4, make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]),
+                                           __uint_as_float(o[i + 3])));
+        }
+        if (!SPLIT && live) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             uint4 w = make_uint4(0, 0, 0, 0);
@@ -724,6 +752,56 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
   }
 }
 
+// Joins a job's parts in their order: a block has 16 rows of a job, a warp one row at a time, HD / 32 columns to a lane.
+constexpr int TJ_ROWS = 16, TJ_THREADS = 128, TL_MAX_SPLITS = 8;
+template <int HD>
+__global__ void __launch_bounds__(TJ_THREADS) tiles_join_kernel(const __grid_constant__ TileParams p) {
+  constexpr int PER = HD / 32;
+  pdl_wait_trigger();
+  const int id = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TileJob job = p.job_of[id];
+  const int head = id % p.a.n_kv_heads;
+  const int n_tok = job.s < p.a.n_seqs ? min(p.tokens_tile, job.span.lq - job.token0) : 0;
+  for (int r = blockIdx.y * TJ_ROWS + warp; r < min(n_tok * p.a.group, (int)(blockIdx.y + 1) * TJ_ROWS); r += TJ_THREADS / 32) {
+    float2 x[TL_MAX_SPLITS];
+    float v[TL_MAX_SPLITS][PER];
+#pragma unroll
+    for (int i = 0; i < TL_MAX_SPLITS; ++i) {
+      const size_t at = ((size_t)id * p.splits + min(i, p.splits - 1)) * TL_M + r;
+      x[i] = __ldcg(p.part_ml + at);
+      if constexpr (PER == 4) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + lane * PER));
+        v[i][0] = y.x, v[i][1] = y.y, v[i][2] = y.z, v[i][3] = y.w;
+      } else {
+        const float2 y = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * HD + lane * PER));
+        v[i][0] = y.x, v[i][1] = y.y;
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < TL_MAX_SPLITS; ++i) {
+      if (i >= p.splits) x[i] = make_float2(-INFINITY, 0.0f);
+      top = fmaxf(top, x[i].x);
+    }
+    const float um = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, acc[PER] = {};
+#pragma unroll
+    for (int i = 0; i < TL_MAX_SPLITS; ++i) {
+      if (x[i].x == -INFINITY && x[i].y == 0.0f) continue;  // a part that saw nothing has put down no output
+      const float f = exp2_fast(x[i].x - um);
+      l += x[i].y * f;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) acc[c] += v[i][c] * f;
+    }
+    const int tok = job.token0 + r / p.a.group, row = job.span.q0 + tok;
+    if (row < 0 || row >= p.a.tokens) continue;  // (what another call left, if this one gave up)
+    const float inv = job.span.lk - job.span.lq + tok + 1 > 0 ? 1.0f / l : 0.0f;
+    __half* to = p.a.out + (long long)row * p.a.so[0] + (long long)(head * p.a.group + r % p.a.group) * p.a.so[1] + lane * PER;
+#pragma unroll
+    for (int c = 0; c < PER; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_half2(acc[c] * inv, acc[c + 1] * inv);
+  }
+}
+
 // Rows of a projection, [64 columns, heads, rows] boxes of a [tokens, heads, head_dim] view.
 int rows_map(adr_ctx* ctx, CUtensorMap* map, const __half* base, const SeqAttention& a, int n_heads, long long s_row,
              long long s_head, int box_heads, int box_rows) {
@@ -734,12 +812,19 @@ int rows_map(adr_ctx* ctx, CUtensorMap* map, const __half* base, const SeqAttent
   return tma_get(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int HD, int NT, bool PAGED>
-int launch_tiles_as(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int min_rows) {
+// Jobs that there can be at most: each sequence fills up its last one.
+long long most_jobs(const SeqAttention& a, int nt) {
+  const long long per = nt * (TL_M / a.group);
+  return std::min<long long>(a.tokens, (a.tokens + a.n_seqs * (per - 1)) / per) * a.n_kv_heads;
+}
+
+template <int HD, int NT, bool PAGED, bool SPLIT>
+int launch_tiles_as(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int min_rows, int splits = 1,
+                    uint8_t* workspace = nullptr) {
   using Cfg = TileCfg<HD, NT>;
-  auto kfn = attention_tiles_kernel<HD, NT, PAGED>;
+  auto kfn = attention_tiles_kernel<HD, NT, PAGED, SPLIT>;
   if (int rc = opt_in_smem(ctx, kfn, Cfg::SMEM); rc != ADR_OK) return rc;
-  TileParams p;
+  TileParams p = {};
   p.a = a;
   p.tokens_tile = TL_M / a.group;
   p.min_rows = min_rows;
@@ -753,25 +838,64 @@ int launch_tiles_as(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, in
     if (int rc = rows_map(ctx, &mk, a.k, a, a.n_kv_heads, a.sk[1], a.sk[2], 1, TL_N); rc != ADR_OK) return rc;
     if (int rc = rows_map(ctx, &mv, a.v, a, a.n_kv_heads, a.sv[1], a.sv[2], 1, TL_N); rc != ADR_OK) return rc;
   }
-  // as many CTAs as there can be: a sequence fills up its last one
-  const long long per = NT * p.tokens_tile;
-  const long long tiles = std::min<long long>(a.tokens, (a.tokens + a.n_seqs * (per - 1)) / per);
-  if (tiles * a.n_kv_heads > 0x7fffffffLL) return ADR_ERR_SHAPE;
-  return launch_whole_sm(ctx, stream, kfn, dim3((unsigned)(tiles * a.n_kv_heads)), Cfg::THREADS, Cfg::SMEM, 1, true, mq,
-                         mk, mv, p);
+  const long long jobs = most_jobs(a, NT);
+  if (jobs > 0x40000000LL) return ADR_ERR_SHAPE;
+  p.splits = splits;
+  if constexpr (SPLIT) {
+    p.job_of = reinterpret_cast<TileJob*>(workspace + TL_JOBS_AT);
+    p.part_ml = reinterpret_cast<float2*>(workspace + TL_PARTS_AT);
+    p.part_o = reinterpret_cast<float*>(p.part_ml + jobs * splits * TL_M);
+  }
+  if (int rc = launch_whole_sm(ctx, stream, kfn, dim3((unsigned)(jobs * splits)), Cfg::THREADS, Cfg::SMEM, 1, true, mq, mk,
+                               mv, p);
+      rc != ADR_OK || !SPLIT)
+    return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)jobs, TL_M / TJ_ROWS);
+  cfg.blockDim = dim3(TJ_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tiles_join_kernel<HD>, p);
+  if (e != cudaSuccess) {
+    ctx->last_cuda_error = (int)e;
+    return ADR_ERR_CUDA;
+  }
+  return after_launch(ctx);
 }
+
+// Parts at once: as many as CTAs that the GPU holds, two to an SM.
+int tile_parts(const adr_ctx* ctx) { return 2 * (ctx->sm_count > 0 ? ctx->sm_count : 148); }
 
 }  // namespace
 
-int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int max_q, int min_rows) {
-  const bool paged = a.block_table != nullptr;
-  const bool one = (long long)max_q * a.group <= TL_M;
-  if (a.head_dim == 128) {
-    if (one) return paged ? launch_tiles_as<128, 1, true>(ctx, stream, a, min_rows) : launch_tiles_as<128, 1, false>(ctx, stream, a, min_rows);
-    return paged ? launch_tiles_as<128, 2, true>(ctx, stream, a, min_rows) : launch_tiles_as<128, 2, false>(ctx, stream, a, min_rows);
+size_t attention_tiles_workspace(const adr_ctx* ctx, int head_dim) {
+  return TL_PARTS_AT + (size_t)tile_parts(ctx) * TL_M * (head_dim + 2) * sizeof(float);
+}
+
+int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int max_q, int min_rows, void* workspace) {
+  // One tile to a CTA and two CTAs to an SM, or two tiles that share their keys.  The former hides one CTA's start and
+  // end behind the other's work, the latter halves what is loaded; measured on 32/32 and 32/8 heads: head_dim 64 in one
+  // tile everywhere (4 x 2048 tokens 135 against 146 us); head_dim 128 of prompts up to 2048 tokens in one (16 x 512: 96
+  // against 111 us, 2 x 6000: 576 against 544), over pages, whose copies are many, up to 512 positions only (16 x 200: 42
+  // against 43 us, 4 x 512 over 1024: 64 against 59).
+  if (a.block_table == nullptr) {
+    if (a.head_dim == 64) return launch_tiles_as<64, 1, false, false>(ctx, stream, a, min_rows);
+    return max_q <= 2048 ? launch_tiles_as<128, 1, false, false>(ctx, stream, a, min_rows)
+                         : launch_tiles_as<128, 2, false, false>(ctx, stream, a, min_rows);
   }
-  if (one) return paged ? launch_tiles_as<64, 1, true>(ctx, stream, a, min_rows) : launch_tiles_as<64, 1, false>(ctx, stream, a, min_rows);
-  return paged ? launch_tiles_as<64, 2, true>(ctx, stream, a, min_rows) : launch_tiles_as<64, 2, false>(ctx, stream, a, min_rows);
+  // Few tiles over many keys: the keys of each are shared out among CTAs, at least four blocks to each.
+  const long long jobs = most_jobs(a, 1), blocks = (long long)a.max_pages * a.page_size / TL_N;
+  const int splits = (int)std::min<long long>({tile_parts(ctx) / std::max(jobs, 1LL), blocks / 4, TL_MAX_SPLITS});
+  if (splits > 1 && (size_t)jobs * sizeof(TileJob) <= TL_PARTS_AT - TL_JOBS_AT)
+    return a.head_dim == 64 ? launch_tiles_as<64, 1, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace)
+                            : launch_tiles_as<128, 1, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace);
+  if (a.head_dim == 64) return launch_tiles_as<64, 1, true, false>(ctx, stream, a, min_rows);
+  return (long long)a.max_pages * a.page_size <= 512 ? launch_tiles_as<128, 1, true, false>(ctx, stream, a, min_rows)
+                                                     : launch_tiles_as<128, 2, true, false>(ctx, stream, a, min_rows);
 }
 
 }  // namespace adr
