@@ -75,7 +75,7 @@ struct Unit {
     }
     return d;
   }
-  __device__ static void store(__half* head, int u, const RopePlan& r, Data d, const float2* turns) {
+  __device__ static void store(__half* head, int u, const RopePlan& r, Data d, const float2 (&turns)[PAIRS]) {
     const int nr = rotated(r.rotary);
     if constexpr (VEC) {
       if (u >= nr) {
@@ -86,7 +86,7 @@ struct Unit {
       __half* y = reinterpret_cast<__half*>(&d.b);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        const float2 w = turns[u * PAIRS + i];
+        const float2 w = turns[i];
         if constexpr (HALF) turn_pair(x[i], y[i], w);
         else turn_pair(x[2 * i], x[2 * i + 1], w);
       }
@@ -98,39 +98,87 @@ struct Unit {
         return;
       }
       __half x = __ushort_as_half((unsigned short)d.a.x), y = __ushort_as_half((unsigned short)d.b.x);
-      turn_pair(x, y, turns[u]);
+      turn_pair(x, y, turns[0]);
       head[HALF ? u : 2 * u] = x;
       head[HALF ? u + r.rotary / 2 : 2 * u + 1] = y;
     }
   }
 };
 
-// Rotates `heads` heads of one row, src to dst (which may be the same), with the turns in shared memory.
-template <bool HALF, bool VEC>
-__device__ __forceinline__ void rotate_heads(__half* dst, long long dst_head, const __half* src, long long src_head,
-                                             int heads, const RopePlan& r, const float2* turns) {
+// A block takes R rows.  With one row each (few rows: latency counts) a thread's first piece is on its way while it is
+// looked up where the row stands, a chain of two or three loads of about a microsecond each; with four the chain and the
+// 64 or so turns of each row are computed by as many threads as there are turns, and each row has two warps of its own.
+// (Single columns, not 16-byte pieces: one row, whose units can be more than two warps.)
+constexpr int ROPE_FEW = 1, ROPE_MANY = 4;
+
+// The place of thread `id` of a row's `threads`: unit u of heads h, h + step, ...  (threads that do not make up a whole
+// head are idle)
+struct Place {
+  int u, h, step;
+  __device__ Place(int per, int id, int threads) : u(id % per), h(id / per), step(threads / per) {
+    if (h >= step) h = 1 << 30;
+  }
+};
+
+// The heads from `at.h` on of one row, two at a time: src_of and dst_of give a head's columns.
+template <bool HALF, bool VEC, typename Src, typename Dst>
+__device__ __forceinline__ void turn_heads(const Place& at, int h, int heads, const RopePlan& r, const float2* turns,
+                                           const Src& src_of, const Dst& dst_of) {
   using U = Unit<HALF, VEC>;
-  const int n = heads * U::count(r.rotary, r.head_dim), per = U::count(r.rotary, r.head_dim);
-  for (int i = threadIdx.x; i < n; i += ROPE_THREADS) {
-    const int h = i / per, u = i - h * per;
-    U::store(dst + h * dst_head, u, r, U::load(src + h * src_head, u, r), turns);
+  float2 w[U::PAIRS];
+  if (at.u < U::rotated(r.rotary) && h < heads) {
+#pragma unroll
+    for (int i = 0; i < U::PAIRS; ++i) w[i] = turns[at.u * U::PAIRS + i];
+  }
+  for (; h < heads; h += 2 * at.step) {
+    const bool two = h + at.step < heads;
+    typename U::Data a = U::load(src_of(h), at.u, r), b;
+    if (two) b = U::load(src_of(h + at.step), at.u, r);
+    U::store(dst_of(h), at.u, r, a, w);
+    if (two) U::store(dst_of(h + at.step), at.u, r, b, w);
   }
 }
+template <bool HALF, bool VEC>
+__device__ __forceinline__ void turn_one(const Place& at, const RopePlan& r, const float2* turns,
+                                         const typename Unit<HALF, VEC>::Data& d, __half* dst) {
+  using U = Unit<HALF, VEC>;
+  float2 w[U::PAIRS];
+#pragma unroll
+  for (int i = 0; i < U::PAIRS; ++i) w[i] = at.u < U::rotated(r.rotary) ? turns[at.u * U::PAIRS + i] : make_float2(1.0f, 0.0f);
+  U::store(dst, at.u, r, d, w);
+}
 
-__device__ __forceinline__ void fill_turns(float2* turns, const RopePlan& r, int position) {
-  for (int i = threadIdx.x; i < r.rotary / 2; i += ROPE_THREADS) turns[i] = turn_at(r, i, position);
+// The turns of R rows, by as many threads as there are.
+template <int R>
+__device__ __forceinline__ void fill_turns(float2 (*turns)[ROPE_MAX_HD / 2], const RopePlan& r, const int* position) {
+  const int n = r.rotary / 2;
+  for (int i = threadIdx.x; i < R * n; i += ROPE_THREADS) turns[i / n][i % n] = turn_at(r, i % n, position[i / n]);
   __syncthreads();
 }
 
-// One row per block.
-template <bool HALF, bool VEC>
-__global__ void __launch_bounds__(ROPE_THREADS)
-    rope_kernel(__half* out, const __half* in, Strided so, Strided si, int heads, const int* positions, RopePlan r) {
-  __shared__ float2 turns[ROPE_MAX_HD / 2];
+// Bound by memory where rows are many (8000 rows of 64 heads of 128: 44 us, 5.9 TB/s).
+template <bool HALF, bool VEC, int R>
+__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(__half* out, const __half* in, Strided so, Strided si, int rows,
+                                                            int heads, const int* positions, RopePlan r) {
+  using U = Unit<HALF, VEC>;
+  __shared__ float2 turns[R][ROPE_MAX_HD / 2];
+  __shared__ int position[R];
   pdl_wait_trigger();
-  const long long t = blockIdx.x;
-  fill_turns(turns, r, __ldg(positions + t));
-  rotate_heads<HALF, VEC>(out + t * so.token, so.head, in + t * si.token, si.head, heads, r, turns);
+  constexpr int ROW_THREADS = ROPE_THREADS / R;
+  const int i = threadIdx.x / ROW_THREADS;  // this thread's row
+  const Place at(U::count(r.rotary, r.head_dim), threadIdx.x % ROW_THREADS, ROW_THREADS);
+  const long long t0 = (long long)blockIdx.x * R;
+  typename U::Data ahead;
+  if (R == 1 && at.h < heads) ahead = U::load(in + t0 * si.token + at.h * si.head, at.u, r);
+  if (threadIdx.x < R) position[threadIdx.x] = __ldg(positions + min(t0 + threadIdx.x, (long long)rows - 1));
+  __syncthreads();
+  fill_turns<R>(turns, r, position);
+  if (t0 + i >= rows) return;
+  const __half* src = in + (t0 + i) * si.token;
+  __half* dst = out + (t0 + i) * so.token;
+  if (R == 1 && at.h < heads) turn_one<HALF, VEC>(at, r, turns[i], ahead, dst + at.h * so.head);
+  turn_heads<HALF, VEC>(at, at.h + (R == 1 ? at.step : 0), heads, r, turns[i], [&](int h) { return src + h * si.head; },
+                        [&](int h) { return dst + h * so.head; });
 }
 
 struct PagePool {
@@ -149,38 +197,70 @@ struct AppendParams {
   unsigned int* status;
 };
 
-template <bool HALF, bool VEC>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(AppendParams p) {
-  __shared__ float2 turns[ROPE_MAX_HD / 2];
+// Four blocks to an SM, 64 registers (8000 rows of 32/8 heads: 66 us against 74 at 72 registers).  Bound by memory: 5.7 TB/s
+// of rows read and written, of 6.55.
+template <bool HALF, bool VEC, int R>
+__global__ void __launch_bounds__(ROPE_THREADS, 4) rope_append_kernel(const __grid_constant__ AppendParams p) {
+  using U = Unit<HALF, VEC>;
+  __shared__ float2 turns[R][ROPE_MAX_HD / 2];
+  __shared__ int position[R], page_of[R];  // page: below 0 there is none, below -1 the row is no sequence's
   pdl_wait_trigger();
-  const int t = blockIdx.x;
-  const int s = find_sequence(p.cu_q, p.n_seqs, t, threadIdx.x & 31);
-  if (s >= p.n_seqs) return;  // rows behind the last sequence
-  const SeqSpan span = seq_span(p.cu_q, nullptr, s, p.tokens, 0, p.status);
-  if (t < span.q0 || t >= span.q0 + span.lq) return;
-  const int position = __ldg(p.kv_len + s) - span.lq + (t - span.q0);
-  fill_turns(turns, p.r, position);
-  rotate_heads<HALF, VEC>(p.q_out + t * p.sqo.token, p.sqo.head, p.q + t * p.sq.token, p.sq.head, p.heads, p.r, turns);
-  int page = -1;
-  if (position >= 0 && position / p.page_size < p.max_pages)
-    page = __ldg(p.block_table + (long long)s * p.max_pages + position / p.page_size);
-  if (page < 0 || page >= p.n_pages) {
-    if (threadIdx.x == 0) atomicOr(p.status, PAGED_BAD);
-    return;
-  }
-  const int slot = position % p.page_size;
-  __half* kd = p.kp.base + page * p.kp.page + slot * p.kp.token;
-  __half* vd = p.vp.base + page * p.vp.page + slot * p.vp.token;
-  rotate_heads<HALF, VEC>(kd, p.kp.head, p.k + t * p.sk.token, p.sk.head, p.kv_heads, p.r, turns);
-  RopePlan copy = p.r;
+  const RopePlan& r = p.r;
+  RopePlan copy = r;
   copy.rotary = 0;
-  rotate_heads<HALF, VEC>(vd, p.vp.head, p.v + t * p.sv.token, p.sv.head, p.kv_heads, copy, turns);
+  constexpr int ROW_THREADS = ROPE_THREADS / R;
+  const int i = threadIdx.x / ROW_THREADS, in_row = threadIdx.x % ROW_THREADS;  // this thread's row
+  const Place at(U::count(r.rotary, r.head_dim), in_row, ROW_THREADS), at_v(U::count(0, r.head_dim), in_row, ROW_THREADS);
+  const int t0 = blockIdx.x * R, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = p.heads + p.kv_heads;
+  // query heads, then key heads
+  auto head_src = [&](long long t, int h) {
+    return h < p.heads ? p.q + t * p.sq.token + h * p.sq.head : p.k + t * p.sk.token + (h - p.heads) * p.sk.head;
+  };
+  typename U::Data ahead;
+  if (R == 1 && at.h < heads) ahead = U::load(head_src(t0, at.h), at.u, r);
+  // a warp looks up one row
+  if (warp < R) {
+    const int t = t0 + warp;
+    int at_position = 0, page = -2;
+    const int s = t < p.tokens ? find_sequence(p.cu_q, p.n_seqs, t, lane) : p.n_seqs;
+    if (s < p.n_seqs) {
+      const int positions = __ldg(p.kv_len + s);
+      const SeqSpan span = seq_span(p.cu_q, nullptr, s, p.tokens, 0, p.status);
+      if (t >= span.q0 && t < span.q0 + span.lq) {
+        at_position = positions - span.lq + (t - span.q0);
+        page = -1;
+        if (at_position >= 0 && at_position / p.page_size < p.max_pages)
+          page = __ldg(p.block_table + (long long)s * p.max_pages + at_position / p.page_size);
+        if (page < 0 || page >= p.n_pages) {
+          page = -1;
+          if (lane == 0) atomicOr(p.status, PAGED_BAD);
+        }
+      }
+    }
+    if (lane == 0) position[warp] = at_position, page_of[warp] = page;
+  }
+  __syncthreads();
+  fill_turns<R>(turns, r, position);
+  const long long t = t0 + i;
+  const int page = page_of[i];
+  if (page < -1) return;
+  const int slot = position[i] % p.page_size;
+  __half* qd = p.q_out + t * p.sqo.token;
+  __half* kd = p.kp.base + (page >= 0 ? page * p.kp.page + slot * p.kp.token : 0);
+  __half* vd = p.vp.base + (page >= 0 ? page * p.vp.page + slot * p.vp.token : 0);
+  const int n = page >= 0 ? heads : p.heads;  // (without a page only the queries)
+  auto head_dst = [&](int h) { return h < p.heads ? qd + h * p.sqo.head : kd + (h - p.heads) * p.kp.head; };
+  if (R == 1 && at.h < n) turn_one<HALF, VEC>(at, r, turns[i], ahead, head_dst(at.h));
+  turn_heads<HALF, VEC>(at, at.h + (R == 1 ? at.step : 0), n, r, turns[i], [&](int h) { return head_src(t, h); }, head_dst);
+  const __half* vs = p.v + t * p.sv.token;
+  turn_heads<HALF, VEC>(at_v, at_v.h, page >= 0 ? p.kv_heads : 0, copy, turns[i], [&](int h) { return vs + h * p.sv.head; },
+                        [&](int h) { return vd + h * p.vp.head; });
 }
 
 template <typename... KArgs, typename... Args>
-int launch_rows(adr_ctx* ctx, cudaStream_t stream, void (*kfn)(KArgs...), int rows, const Args&... args) {
+int launch_rows(adr_ctx* ctx, cudaStream_t stream, void (*kfn)(KArgs...), int blocks, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows);
+  cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(ROPE_THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -194,10 +274,14 @@ int launch_rows(adr_ctx* ctx, cudaStream_t stream, void (*kfn)(KArgs...), int ro
     return ADR_ERR_CUDA;
   }
   // (as for the other row kernels: with a block per SM and more it fills the GPU)
-  if (rows >= ctx->sm_count) note_filling_launch(ctx, stream, 4);
+  if (blocks >= ctx->sm_count) note_filling_launch(ctx, stream, 4);
   else ctx->small_before = 1;
   return after_launch(ctx);
 }
+
+// From two rows to an SM on they go four to a block (600 rows of 32/8 heads: 5.7 against 8.3 us; 148 rows would take 4.0 either
+// way, and below that the single rows' first loads are worth more).
+bool many_rows(const adr_ctx* ctx, int rows) { return rows >= 2 * ctx->sm_count; }
 
 int check_rotation(const uint64_t* turns, int head_dim, int rotary_dim, float amplitude, uint32_t layout) {
   if (!turns || head_dim <= 0 || rotary_dim <= 0 || layout > ADR_ROPE_HALF) return ADR_ERR_INVALID;
@@ -286,10 +370,14 @@ extern "C" int adr_rope_f16(adr_ctx* ctx, adr_stream stream, void* out, const vo
                    in_pieces(in, strides_i, 2);
   const RopePlan r{reinterpret_cast<const unsigned long long*>(turns), rotary_dim, amplitude, head_dim};
   const Strided so{strides_o[0], strides_o[1]}, si{strides_i[0], strides_i[1]};
-  auto kfn = layout == ADR_ROPE_HALF ? (vec ? rope_kernel<true, true> : rope_kernel<true, false>)
-                                     : (vec ? rope_kernel<false, true> : rope_kernel<false, false>);
-  return launch_rows(ctx, (cudaStream_t)stream, kfn, tokens, (__half*)out, (const __half*)in, so, si, n_heads,
-                     (const int*)positions, r);
+  auto go = [&](auto kfn, int per) {
+    return launch_rows(ctx, (cudaStream_t)stream, kfn, (tokens + per - 1) / per, (__half*)out, (const __half*)in, so, si,
+                       tokens, n_heads, (const int*)positions, r);
+  };
+  const bool many = vec && many_rows(ctx, tokens), half = layout == ADR_ROPE_HALF;
+  if (many) return half ? go(rope_kernel<true, true, ROPE_MANY>, ROPE_MANY) : go(rope_kernel<false, true, ROPE_MANY>, ROPE_MANY);
+  if (vec) return half ? go(rope_kernel<true, true, ROPE_FEW>, ROPE_FEW) : go(rope_kernel<false, true, ROPE_FEW>, ROPE_FEW);
+  return half ? go(rope_kernel<true, false, ROPE_FEW>, ROPE_FEW) : go(rope_kernel<false, false, ROPE_FEW>, ROPE_FEW);
 }
 
 extern "C" int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_out, const void* q, const void* k,
@@ -337,7 +425,11 @@ extern "C" int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_ou
   p.n_pages = n_pages;
   p.r = {reinterpret_cast<const unsigned long long*>(turns), rotary_dim, amplitude, head_dim};
   p.status = ctx->d_status;
-  auto kfn = layout == ADR_ROPE_HALF ? (vec ? rope_append_kernel<true, true> : rope_append_kernel<true, false>)
-                                     : (vec ? rope_append_kernel<false, true> : rope_append_kernel<false, false>);
-  return launch_rows(ctx, (cudaStream_t)stream, kfn, tokens, p);
+  auto go = [&](auto kfn, int per) { return launch_rows(ctx, (cudaStream_t)stream, kfn, (tokens + per - 1) / per, p); };
+  const bool many = vec && many_rows(ctx, tokens), half = layout == ADR_ROPE_HALF;
+  if (many)
+    return half ? go(rope_append_kernel<true, true, ROPE_MANY>, ROPE_MANY) : go(rope_append_kernel<false, true, ROPE_MANY>, ROPE_MANY);
+  if (vec)
+    return half ? go(rope_append_kernel<true, true, ROPE_FEW>, ROPE_FEW) : go(rope_append_kernel<false, true, ROPE_FEW>, ROPE_FEW);
+  return half ? go(rope_append_kernel<true, false, ROPE_FEW>, ROPE_FEW) : go(rope_append_kernel<false, false, ROPE_FEW>, ROPE_FEW);
 }

@@ -498,7 +498,7 @@ int adr_attention_f16(adr_ctx* ctx, adr_stream stream, void* out, const void* q,
  * at a time, llama.rs:426-427).  Three arrays in device memory describe the batch, so that a
  * captured step can be replayed with other lengths:
  *   cu_q [n_seqs + 1]  the rows of sequence s are cu_q[s] .. cu_q[s + 1] - 1 (not decreasing; a
- *                      sequence may have none); rows of no sequence are neither read nor written;
+ *                      sequence may have none); nothing is written for rows of no sequence;
  *   kv_len [n_seqs]    positions of sequence s with its new rows, which are the last of them: row i
  *                      of lq is at position kv_len[s] - lq + i;
  *   block_table [n_seqs, max_pages]  position p lies in slot p % page_size of page
