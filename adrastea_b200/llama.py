@@ -13,7 +13,8 @@ Differences from the reference, which re-runs the whole prefix for every token
 (llama.rs:426-427): a KV cache ([B, S, heads*head_dim] per layer) with the two
 decode kernels that serve it (`decode_rope_append`, `decode_attention`), batches of
 sequences, q/k/v and gate/up stored as one matrix each (one GEMV instead of three
-or two; the separate matrices remain available as row slices), tensor parallelism
+or two; the separate matrices remain available as row slices), sequences of different lengths over a
+paged cache (`PagedCache`, `LlamaU8.extend`), tensor parallelism
 (adrastea_b200/tp.py) and CUDA-graph capture of the decode step are harness glue
 that the LLaMA-7B and 65B-shape decode workloads need.  Weights are seeded random u8 codes with
 the config-2 distributions; there are no checkpoints in this environment.
@@ -82,6 +83,43 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, n_heads: int, theta: float) -> to
 def _rows(w: U8Weight, lo: int, hi: int) -> U8Weight:
     """Rows [lo, hi) of a quantised matrix as a view (no copy)."""
     return U8Weight(w.q[lo:hi], w.scales[lo:hi], w.block, None if w.zeros is None else w.zeros[lo:hi])
+
+
+class PagedCache:
+    """A pool of key and value pages for all layers ([layers, pages, page_size, heads, head_dim]) and the
+    pages of every sequence.  Pages are handed out as sequences grow and come back with `release`; the
+    block table lives on the device, one row per sequence slot, and is written only where it changes."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, heads: int, head_dim: int, max_seqs: int,
+                 max_positions: int, device: str | torch.device = "cuda"):
+        self.page_size, self.device = page_size, torch.device(device)
+        self.max_pages = -(-max_positions // page_size)
+        f16 = dict(dtype=torch.float16, device=self.device)
+        self.k = torch.zeros((layers, pages, page_size, heads, head_dim), **f16)
+        self.v = torch.zeros((layers, pages, page_size, heads, head_dim), **f16)
+        self.table = torch.full((max_seqs, self.max_pages), -1, dtype=torch.int32, device=self.device)
+        self.free = list(range(pages - 1, -1, -1))
+        self.pages: list[list[int]] = [[] for _ in range(max_seqs)]
+        self.length = [0] * max_seqs
+
+    def extend(self, seqs: list[int], new: list[int]):
+        """Room for new[i] more positions of sequence slot seqs[i]; all of them, or MemoryError and none."""
+        assert len(set(seqs)) == len(seqs) == len(new) and min(new) >= 0
+        need = [-(-(self.length[s] + n) // self.page_size) - len(self.pages[s]) for s, n in zip(seqs, new)]
+        if any(self.length[s] + n > self.max_pages * self.page_size for s, n in zip(seqs, new)):
+            raise MemoryError("a sequence is longer than its row of the block table")
+        if sum(need) > len(self.free):
+            raise MemoryError(f"{sum(need)} pages wanted, {len(self.free)} free")
+        for s, n, m in zip(seqs, new, need):
+            if m > 0:
+                at, got = len(self.pages[s]), [self.free.pop() for _ in range(m)]
+                self.pages[s] += got
+                self.table[s, at:at + m] = torch.tensor(got, dtype=torch.int32, device=self.device)
+            self.length[s] += n
+
+    def release(self, seq: int):
+        self.free += reversed(self.pages[seq])
+        self.pages[seq], self.length[seq] = [], 0
 
 
 class LlamaU8Layer:
@@ -155,6 +193,7 @@ class LlamaU8:
         self.fused_attention = hd in (64, 128) and dl % 8 == 0  # what adr_attention_f16 takes
         self._graph = None
         self._deq = None  # fp16 scratch for one expanded weight matrix (prefill)
+        self._rope = self._attention_ws = None  # table and workspace of `extend`
         # rms_norm inside the decode product that follows it (adr_rms_norm_matmul_nt_fp16u8,
         # adr_rms_norm_silu_mul_matmul_nt_fp16u8: same bits, one launch fewer per norm), for the
         # batches of up to four that run on that kernel: 16 layers of the 7B shape at 575 positions
@@ -395,6 +434,54 @@ class LlamaU8:
         self.k.matmul_nt_fp16u8(self.logits, self.x, self.lm_head.q, self.lm_head.scales, self.lm_head.block)
         self.tokens.copy_(torch.argmax(self.logits, dim=-1))
         self.pos.fill_(S0)
+
+
+    # --------------------------------------------- sequences of different lengths
+    def paged_cache(self, pages: int, page_size: int = 64, max_seqs: int | None = None,
+                    max_positions: int | None = None) -> PagedCache:
+        """A cache for `extend`; slots for max_batch sequences of max_seq positions unless said otherwise."""
+        return PagedCache(self.L, pages, page_size, self.Hl, self.shape.head_dim, max_seqs or self.B,
+                          max_positions or self.S, self.device)
+
+    def extend(self, cache: PagedCache, seqs: list[int], tokens: list[torch.Tensor]) -> torch.Tensor:
+        """tokens[i] (int64, at least one) go behind what the cache holds of sequence slot seqs[i]: whole prompts,
+        chunks of them and single tokens in any mixture, all rows through each layer at once.  Returns the argmax
+        behind every sequence's last token; self.logits[:len(seqs)] holds the logits."""
+        sh, n = self.shape, len(seqs)
+        assert 0 < n <= self.B and self.fused_attention and all(t.numel() > 0 for t in tokens)
+        new = [t.numel() for t in tokens]
+        cache.extend(seqs, new)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=self.device)
+        starts = [0]
+        for m in new:
+            starts.append(starts[-1] + m)
+        T, hd, Hl, d, dl, fl = starts[-1], sh.head_dim, self.Hl, sh.dim, self.dl, self.fl
+        cu_q, kv_len, table = ints(starts), ints([cache.length[s] for s in seqs]), cache.table[seqs]
+        if self._rope is None:
+            self._rope = self.k.rope_table(hd, sh.theta)
+            self._attention_ws = self.k.attention_paged_workspace(Hl, Hl, hd)
+        f16 = dict(dtype=torch.float16, device=self.device)
+        h = self.embed[torch.cat([t.reshape(-1) for t in tokens])].clone()
+        x, part = torch.empty((T, d), **f16), torch.zeros((T, d), **f16) if self.tp.world > 1 else None
+        qkv, att = torch.zeros((T, 3 * dl), **f16), torch.empty((T, dl), **f16)   # (zeros: see prefill)
+        gu, g = torch.zeros((T, 2 * fl), **f16), torch.empty((T, fl), **f16)
+        heads = lambda t: TensorView.of(t.unflatten(1, (Hl, hd)))
+        q, k, v = (heads(t) for t in qkv.split(dl, 1))
+        for li, ly in enumerate(self.layers):
+            self._norm(x, h, ly.attn_norm)
+            self._prefill_linear(ly.wqkv, qkv, x)
+            self.k.rope_append_paged(q, q, k, v, cache.k[li], cache.v[li], table, cu_q, kv_len, self._rope)
+            self.k.attention_paged(heads(att), q, cache.k[li], cache.v[li], table, cu_q, kv_len, max(new),
+                                   1.0 / math.sqrt(hd), self._attention_ws)
+            self._prefill_linear(ly.wo, h, att, part, residual=True)
+            self._norm(x, h, ly.ffn_norm)
+            self._prefill_linear(ly.wgu, gu, x)
+            self._silu_mul(g, gu)
+            self._prefill_linear(ly.down, h, g, part, residual=True)
+        last = h[cu_q[1:].long() - 1]
+        self._norm(self.x[:n], last, self.out_norm)
+        self.k.matmul_nt_fp16u8(self.logits[:n], self.x[:n], self.lm_head.q, self.lm_head.scales, self.lm_head.block)
+        return torch.argmax(self.logits[:n], dim=-1)
 
 
 def main():
