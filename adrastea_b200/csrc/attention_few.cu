@@ -749,9 +749,9 @@ int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, cons
   const int ctas = (int)std::min<double>(g, units);
   if (int rc = launch_whole_sm(ctx, stream, kfn, dim3(ctas), FEW_THREADS, Cfg::SMEM, 1, true, mk, mv, p); rc != ADR_OK)
     return rc;
-  // the borders between the chunks: none where a CTA is all there is
+  // the borders between the chunks: none where a CTA is all there is, and none inside an item of one block
   const int borders = (int)std::min<double>(ctas * (1 + Cfg::SPARE), units) - 1;
-  if (borders < 1) return ADR_OK;
+  if (borders < 1 || (long long)p.a.max_pages * p.a.page_size <= FEW_KB) return ADR_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(borders);
   cfg.blockDim = dim3(JOIN_THREADS);

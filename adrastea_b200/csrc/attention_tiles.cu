@@ -512,11 +512,12 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       auto look_at_values = [&] {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[(2 * j + 1) % SLOTS], (unsigned)((2 * j + 1) / SLOTS) & 1u));
         const int from = max(0, all_see - key0), end = min(TL_N, lk - key0);
+        const int read = min(TL_N, (my_end - key0 + 15) & ~15);  // rows that the tensor cores read
         constexpr int LPR = HD / 8, STEP = 128 / LPR;
         uint4* at = reinterpret_cast<uint4*>(v + ((row % LPR) / 8) * (TL_N * 128) + (row % 8) * 16);
         uint32_t odd = 0;
         int r = from + row / LPR;
-        for (; r + 3 * STEP < end; r += 4 * STEP) {
+        for (; r + 3 * STEP < min(end, read); r += 4 * STEP) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint4 x = at[(r + i * STEP) * 8];
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
           }
         }
 #pragma unroll 1
-        for (; r < TL_N; r += STEP) {
+        for (; r < read; r += STEP) {
           if (r >= end) {
             at[r * 8] = make_uint4(0, 0, 0, 0);
           } else {
@@ -535,13 +536,13 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         fence_proxy_async();
         hand = tile_any(t, odd != 0);
       };
-      // While the scores are computed; but a barrier's phase may be waited for only when the one before it is known to be
-      // complete, and with two slots that one is the V before, whose product the scores come behind.
+      // While the scores are computed; but with two slots a block's V is loaded only when the product with the one before
+      // is done: it is looked at behind the probabilities then.  (Nor may it be waited for before the scores: a barrier's
+      // phase can be told from the next but one only when the one between is known to be complete.)
       const bool early = SLOTS > 2 || j == 0;
       if (partly && early) look_at_values();
       if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_s, (unsigned)j & 1u));
       tc_fence_after_sync();
-      if (partly && !early) look_at_values();
       if (ok && warp_live) {
         const int chunks = partly ? (min(TL_N, my_end - key0) + 31) / 32 : 4;  // of 32 keys
         // the row's maximum
@@ -654,6 +655,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         l += total.x + total.y;
       }
       tmem_wait_st();
+      if (partly && !early) look_at_values();
       if (hand && ok && warp_live) {
         // this block's product by hand
         const int end = min(TL_N, my_end - key0);
