@@ -1,17 +1,18 @@
 // Attention of a few new rows per sequence over a paged cache: single tokens, and a few at a time.
 //
-// The rows of one key head (its query heads times the new tokens, up to 64) share every key and value, so one pass
+// The rows of one key head (its query heads times the new tokens, up to 32) share every key and value, so one pass
 // over the cache serves them all: what bounds this kernel is reading the cache once.
-//   * Work is counted in units of 64 keys of one (sequence, key head, tile of rows) and cut into chunks by the lengths
+//   * Work is counted in units of 64 keys (of 128 columns; 128 of 64) of one (sequence, key head, tile of rows) and cut into chunks by the lengths
 //     on the device, so the cache of a batch of very different lengths, or of one long sequence, is spread evenly with
-//     no plan from the host.  Every CTA has one chunk of its own, 80 % of an even share; the rest lies in small chunks
+//     no plan from the host.  Every CTA has one chunk of its own, 7/8 of an even share; the rest lies in small chunks
 //     that CTAs take as they get done (SMs do not get equal shares of the memory's bandwidth: with even shares the
 //     slowest of 296 CTAs was done after 94 us where the median one took 77).
-//   * The producer warp looks up what comes next and copies pages by TMA into a ring of stages (64 keys and values),
+//   * The producer warp looks up what comes next and copies pages by TMA into a ring of stages (a unit's keys and values),
 //     across the borders of items.
-//   * Four warps compute: S = Q K^T and O += P V by mma.sync m16n8k16 with the 16 (32, 64) rows as M and a running
+//   * Four warps compute: S = Q K^T and O += P V by mma.sync m16n8k16 with the 16 (32) rows as M and a running
 //     maximum and sum.  (tcgen05 wants 64 or 128 rows: at up to 16 live ones the tensor work is 5 % of the time that
-//     the keys take to arrive.)  With 16 rows the warps share a stage's keys, with 64 its rows.
+//     the keys take to arrive.  With 64 rows, a row tile to each warp, this kernel took 1.3 to 2.5 times what the tiles of
+//     attention_tiles.cu take.)  With 16 rows the warps share a stage's keys among them, with 32 two by two.
 //   * An item that lies within one chunk is finished there.  Otherwise each part stores its maximum, sum and unscaled
 //     output, and a second kernel, which is resident before the first one ends, joins them in their order.  (Joined by
 //     the CTA that came last, 111 parts took 65 us: a join is a chain of loads of about a microsecond each, and one CTA
@@ -24,22 +25,26 @@ namespace adr {
 
 namespace {
 
-constexpr int FEW_KB = 64;          // keys of a stage, and of a unit of work
 constexpr int FEW_THREADS = 160;    // four computing warps and the producer
+
+constexpr int few_kb(int head_dim) { return 8192 / head_dim; }  // 64 keys of 128 columns, 128 of 64
 
 template <int HD, int WM>
 struct FewCfg {
+  static constexpr int KB = few_kb(HD);         // keys of a stage, and of a unit of work
   static constexpr int ROWS = 16 * WM;
   static constexpr int WK = 4 / WM;             // warps that share a stage's keys
-  static constexpr int KEYS = FEW_KB / WK;      // of a stage, for one warp
+  static constexpr int KEYS = KB / WK;          // of a stage, for one warp
+  static constexpr int SK = KEYS < 32 ? KEYS : 32;  // of a step of a warp
   static constexpr int CH = HD / 64;            // 64-column chunks of a head
-  static constexpr int TILE = FEW_KB * HD * 2;  // bytes of a stage's keys
-  static constexpr int STAGES = HD == 128 ? 3 : 6;
+  static constexpr int TILE = KB * HD * 2;      // bytes of a stage's keys: 16 KB
+  static constexpr int STAGES = 3;
   static constexpr int MERGE = WK == 1 ? 0 : 4 * (HD / 8) * 32 * 8;  // eight rows of every warp
   static constexpr int SEGS = STAGES + 2;       // descriptors in flight (a segment has at least one stage)
   static constexpr size_t SMEM = (size_t)STAGES * 2 * TILE + MERGE + 4 * 16 * 8 + 16 * STAGES + 8 * SEGS +
                                  SEGS * 48;
-  static constexpr int SPARE = WM == 1 ? 2 : 1; // small chunks per CTA
+  static constexpr int SPARE = WM == 1 ? 2 : 1;  // small chunks per CTA
+  static_assert(WM == 1 || WM == 2, "");
 };
 
 struct Segment;
@@ -47,7 +52,7 @@ struct Segment;
 struct FewParams {
   SeqAttention a;
   int max_rows;  // sequences with more rows of a key head than this are left to another kernel
-  int page_rows; // rows of a copy: a page, 64 at most
+  int page_rows; // rows of a copy: a page, a stage at most
   int min_units; // of a CTA, where there are few
   int spare, spare_units;  // small chunks per CTA where a share has at least spare_units units
   float* part_ml;          // [slots][ROWS][2]: two slots to a chunk
@@ -92,7 +97,7 @@ __device__ __forceinline__ bool few_all(bool x) {
   return r != 0;
 }
 
-// Where in the list of all units (sequence by sequence, key head by key head, tile by tile, 64 keys each) one is.
+// Where in the list of all units (sequence by sequence, key head by key head, tile by tile, KB keys each) one is.
 struct Walk {
   SeqSpan span;
   int s, head, tile, blk;
@@ -105,7 +110,7 @@ struct Share {
   int total, ctas, spare;
   int per, more;      // units of a span (the first `more` spans have one more)
   __device__ int span_begin(int c) const { return c * per + min(c, more); }
-  __device__ int own(int size) const { return spare ? size - size / 5 : size; }
+  __device__ int own(int size) const { return spare ? size - size / 8 : size; }
   __device__ int2 range(int chunk) const {
     if (chunk < ctas) {
       const int b = span_begin(chunk);
@@ -147,7 +152,7 @@ struct Segment {
 };
 static_assert(sizeof(Segment) == 48, "");
 
-template <int ROWS>
+template <int ROWS, int KB>
 struct FewWork {
   const FewParams& p;
   const int lane, q;  // a lane stands for q sequences
@@ -173,7 +178,7 @@ struct FewWork {
     const long long rows = (long long)v.lq * p.a.group;
     return rows > p.max_rows ? 0 : (int)((rows + ROWS - 1) / ROWS);
   }
-  __device__ static int blocks(const SeqSpan& v) { return max(1, (v.lk + FEW_KB - 1) / FEW_KB); }
+  __device__ static int blocks(const SeqSpan& v) { return max(1, (v.lk + KB - 1) / KB); }
   __device__ int units(int s) const {
     if (s >= p.a.n_seqs) return 0;
     const SeqSpan v = span(s);
@@ -185,7 +190,7 @@ struct FewWork {
     r.ctas = min((int)gridDim.x, (r.total + p.min_units - 1) / p.min_units);
     r.per = r.ctas ? r.total / r.ctas : 0;
     r.more = r.total - r.per * r.ctas;
-    r.spare = r.per >= max(p.spare_units, 5 * p.spare) ? p.spare : 0;  // (no small chunk may be empty)
+    r.spare = r.per >= max(p.spare_units, 8 * p.spare) ? p.spare : 0;  // (no small chunk may be empty)
     return r;
   }
   __device__ void enter(Walk& w, int s) const {
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   if (warp == 4) {
     // ------------------------------- producer -------------------------------
     // It alone looks up what is to be done, so that the warps that meet at barriers agree on it.
-    const FewWork<Cfg::ROWS> work(p, lane);
+    const FewWork<Cfg::ROWS, Cfg::KB> work(p, lane);
     const Share share = work.share();
     const int pr = p.page_rows, page_size = p.a.page_size;
     int st = 0, issued = 0, seg = 0;
@@ -407,9 +412,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         if (u == range.x && lane == 0) p.begins[place] = g;
         const int* row = p.a.block_table + (long long)w.s * p.a.max_pages;
         for (int b = w.blk; b < last; ++b) {
-          const int keys = min(FEW_KB, w.span.lk - b * FEW_KB);
+          const int keys = min(Cfg::KB, w.span.lk - b * Cfg::KB);
           const int copies = (max(keys, 0) + pr - 1) / pr;  // none: a sequence without positions
-          const int pos = b * FEW_KB + lane * pr;
+          const int pos = b * Cfg::KB + lane * pr;
           int page = 0;
           if (lane < copies) {
             page = __ldg(row + pos / page_size);
@@ -427,8 +432,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
             const int slot = pos % page_size;
 #pragma unroll
             for (int c = 0; c < Cfg::CH; ++c) {
-              tma_load_4d(k_sm + c * FEW_KB * 128, &map_k, c * 64, w.head, slot, page, &full[st]);
-              tma_load_4d(k_sm + Cfg::TILE + c * FEW_KB * 128, &map_v, c * 64, w.head, slot, page, &full[st]);
+              tma_load_4d(k_sm + c * Cfg::KB * 128, &map_k, c * 64, w.head, slot, page, &full[st]);
+              tma_load_4d(k_sm + Cfg::TILE + c * Cfg::KB * 128, &map_v, c * 64, w.head, slot, page, &full[st]);
             }
           }
           ++issued;
@@ -508,27 +513,30 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       const uint32_t k_sm = smem_u32(ring + (size_t)st * 2 * Cfg::TILE);
       const uint32_t v_sm = k_sm + Cfg::TILE;
 #pragma unroll 1
-      for (int step = 0; step < Cfg::KEYS; step += 16) {
+      for (int step = 0; step < Cfg::KEYS; step += Cfg::SK) {
         const int kb = wk * Cfg::KEYS + step;  // of the stage
-        const int key0 = b * FEW_KB + kb;      // position of its first key
+        const int key0 = b * Cfg::KB + kb;      // position of its first key
         if (key0 >= lk) break;
-        float s[2][4];
+        constexpr int SK = Cfg::SK, G = SK / 16;
+        float s[2 * G][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2 * G; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][i] = 0.0f;
         const uint32_t k_row = k_sm + (kb + k_key) * 128;
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          uint32_t kf[4];
-          ldsm_x4(k_row + (kk / 4) * FEW_KB * 128 + ((((kk & 3) * 2 + k_col) ^ (k_key & 7)) << 4), kf);
-          mma_16816(s[0], qa[kk], kf[0], kf[1]);
-          mma_16816(s[1], qa[kk], kf[2], kf[3]);
-        }
-        const bool partly = key0 + 16 > all_see;  // some row does not see some of these keys
+        for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            uint32_t kf[4];
+            ldsm_x4(k_row + g * 16 * 128 + (kk / 4) * Cfg::KB * 128 + ((((kk & 3) * 2 + k_col) ^ (k_key & 7)) << 4), kf);
+            mma_16816(s[2 * g], qa[kk], kf[0], kf[1]);
+            mma_16816(s[2 * g + 1], qa[kk], kf[2], kf[3]);
+          }
+        const bool partly = key0 + SK > all_see;  // some row does not see some of these keys
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2 * G; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             s[t][i] *= scale2;
@@ -556,75 +564,89 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
           l[1] *= alpha[1];
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2 * G; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             s[t][i] = exp2_fast(s[t][i] - use_m[i >> 1]);
             l[i >> 1] += s[t][i];
           }
         // probabilities are rounded to fp16 for the tensor cores (2^-11 of each: as much as the output's own rounding)
-        const uint32_t pa[4] = {pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]),
-                                pack_half2(s[1][0], s[1][1]), pack_half2(s[1][2], s[1][3])};
+        uint32_t pa[G][4];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          pa[g][0] = pack_half2(s[2 * g][0], s[2 * g][1]), pa[g][1] = pack_half2(s[2 * g][2], s[2 * g][3]);
+          pa[g][2] = pack_half2(s[2 * g + 1][0], s[2 * g + 1][1]), pa[g][3] = pack_half2(s[2 * g + 1][2], s[2 * g + 1][3]);
+        }
         const uint32_t v_row = v_sm + (kb + v_key) * 128;
-        auto v_addr = [&](int d16) {
-          return v_row + (d16 / 4) * FEW_KB * 128 + ((((d16 & 3) * 2 + v_col) ^ (v_key & 7)) << 4);
+        auto v_addr = [&](int g, int d16) {
+          return v_row + g * 16 * 128 + (d16 / 4) * Cfg::KB * 128 + ((((d16 & 3) * 2 + v_col) ^ (v_key & 7)) << 4);
         };
         if (!partly) {
 #pragma unroll
-          for (int d = 0; d < HD / 16; ++d) {
-            uint32_t vf[4];
-            ldsm_x4_t(v_addr(d), vf);
-            mma_16816(o[2 * d], pa, vf[0], vf[1]);
-            mma_16816(o[2 * d + 1], pa, vf[2], vf[3]);
-          }
+          for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              uint32_t vf[4];
+              ldsm_x4_t(v_addr(g, d), vf);
+              mma_16816(o[2 * d], pa[g], vf[0], vf[1]);
+              mma_16816(o[2 * d + 1], pa[g], vf[2], vf[3]);
+            }
           continue;
         }
         // A probability of zero does not silence a value that is infinite or not a number.  Values behind the last
         // position (whatever the page holds there) are cleared; if one that only some rows see is not finite, the
-        // step is done key by key, for the rows that see it.
-        uint32_t keep[2], odd = 0;
+        // sixteen keys are done one by one, for the rows that see them.
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int key = key0 + pairc + 8 * i;
-          keep[i] = (key < lk ? 0xFFFFu : 0u) | (key + 1 < lk ? 0xFFFF0000u : 0u);
-        }
-        if (all_see < min(lk, key0 + 16)) {
-#pragma unroll 1
-          for (int d = 0; d < HD / 16; ++d) {
-            uint32_t vf[4];
-            ldsm_x4_t(v_addr(d), vf);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) odd |= not_finite2(vf[i] & keep[i & 1]);
-          }
-        }
-        if (!__any_sync(0xffffffffu, odd != 0)) {
-#pragma unroll
-          for (int d = 0; d < HD / 16; ++d) {
-            uint32_t vf[4];
-            ldsm_x4_t(v_addr(d), vf);
-            mma_16816(o[2 * d], pa, vf[0] & keep[0], vf[1] & keep[1]);
-            mma_16816(o[2 * d + 1], pa, vf[2] & keep[0], vf[3] & keep[1]);
-          }
-          continue;
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const int from = (lane & ~3) | ((k & 7) >> 1);
-          float pk[2];
+        for (int g = 0; g < G; ++g) {
+          const int first = key0 + 16 * g;
+          if (first >= lk) break;
+          uint32_t keep[2], odd = 0;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float x = __shfl_sync(0xffffffffu, s[k >> 3][2 * i + (k & 1)], from);
-            pk[i] = __half2float(__float2half_rn(x));
+            const int key = first + pairc + 8 * i;
+            keep[i] = (key < lk ? 0xFFFFu : 0u) | (key + 1 < lk ? 0xFFFF0000u : 0u);
           }
-          const bool see0 = key0 + k < limit[0], see1 = key0 + k < limit[1];
+          if (all_see < min(lk, first + 16)) {
+#pragma unroll 1
+            for (int d = 0; d < HD / 16; ++d) {
+              uint32_t vf[4];
+              ldsm_x4_t(v_addr(g, d), vf);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            uint32_t raw;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(raw)
-                         : "r"(v_sm + (kb + k) * 128 + (t / 8) * FEW_KB * 128 + (((t & 7) ^ ((kb + k) & 7)) << 4) + pairc * 2));
-            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&raw));
-            if (see0) o[t][0] = fmaf(pk[0], v.x, o[t][0]), o[t][1] = fmaf(pk[0], v.y, o[t][1]);
-            if (see1) o[t][2] = fmaf(pk[1], v.x, o[t][2]), o[t][3] = fmaf(pk[1], v.y, o[t][3]);
+              for (int i = 0; i < 4; ++i) odd |= not_finite2(vf[i] & keep[i & 1]);
+            }
+          }
+          if (!__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) {
+              uint32_t vf[4];
+              ldsm_x4_t(v_addr(g, d), vf);
+              mma_16816(o[2 * d], pa[g], vf[0] & keep[0], vf[1] & keep[1]);
+              mma_16816(o[2 * d + 1], pa[g], vf[2] & keep[0], vf[3] & keep[1]);
+            }
+            continue;
+          }
+#pragma unroll 1
+          for (int k = 0; k < 16; ++k) {
+            const int from = (lane & ~3) | ((k & 7) >> 1);
+            float pk[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float even = k < 8 ? s[2 * g][2 * i] : s[2 * g + 1][2 * i];
+              const float uneven = k < 8 ? s[2 * g][2 * i + 1] : s[2 * g + 1][2 * i + 1];
+              const float x = __shfl_sync(0xffffffffu, (k & 1) ? uneven : even, from);
+              pk[i] = __half2float(__float2half_rn(x));
+            }
+            const int at = kb + 16 * g + k;
+            const bool see0 = first + k < limit[0], see1 = first + k < limit[1];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              uint32_t raw;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(raw)
+                           : "r"(v_sm + at * 128 + (t / 8) * Cfg::KB * 128 + (((t & 7) ^ (at & 7)) << 4) + pairc * 2));
+              const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+              if (see0) o[t][0] = fmaf(pk[0], v.x, o[t][0]), o[t][1] = fmaf(pk[0], v.y, o[t][1]);
+              if (see1) o[t][2] = fmaf(pk[1], v.x, o[t][2]), o[t][3] = fmaf(pk[1], v.y, o[t][3]);
+            }
           }
         }
       }
@@ -751,7 +773,7 @@ int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, cons
     return rc;
   // the borders between the chunks: none where a CTA is all there is, and none inside an item of one block
   const int borders = (int)std::min<double>(ctas * (1 + Cfg::SPARE), units) - 1;
-  if (borders < 1 || (long long)p.a.max_pages * p.a.page_size <= FEW_KB) return ADR_OK;
+  if (borders < 1 || (long long)p.a.max_pages * p.a.page_size <= Cfg::KB) return ADR_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(borders);
   cfg.blockDim = dim3(JOIN_THREADS);
@@ -771,9 +793,10 @@ int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, cons
 
 // What the units of the launch can be at most: tiles of `rows` rows, blocks of the longest table row.
 double few_units(const SeqAttention& a, int rows, bool one_tile_each) {
-  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  const int tile = rows <= 16 ? 16 : 32;
   const double tiles = one_tile_each ? a.n_seqs : (double)a.tokens * a.group / tile + a.n_seqs;
-  const double blocks = (double)(((long long)a.max_pages * a.page_size + FEW_KB - 1) / FEW_KB);
+  const int kb = few_kb(a.head_dim);
+  const double blocks = (double)(((long long)a.max_pages * a.page_size + kb - 1) / kb);
   return tiles * blocks * a.n_kv_heads;
 }
 
@@ -781,7 +804,7 @@ double few_units(const SeqAttention& a, int rows, bool one_tile_each) {
 
 size_t attention_few_workspace(const adr_ctx* ctx, int head_dim) {
   const size_t g = few_ctas(ctx);
-  const size_t rows = std::max({few_rows<128, 1>(g), few_rows<128, 2>(g), few_rows<128, 4>(g)});
+  const size_t rows = std::max(few_rows<128, 1>(g), few_rows<128, 2>(g));
   return FEW_HEAD + few_begins(g) + rows * (head_dim + 2) * sizeof(float);
 }
 
@@ -794,8 +817,8 @@ int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& 
   p.a = a;
   p.max_rows = max_rows;
   p.min_units = std::max(1, ctx->tune_att_cs.load());
-  p.spare_units = 16;
-  p.page_rows = a.page_size < FEW_KB ? a.page_size : FEW_KB;
+  p.spare_units = 32;
+  p.page_rows = std::min(a.page_size, few_kb(a.head_dim));
   uint8_t* at = static_cast<uint8_t*>(workspace);
   p.queue = reinterpret_cast<unsigned int*>(at);
   p.begins = reinterpret_cast<Segment*>(at + FEW_HEAD);
@@ -803,14 +826,10 @@ int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& 
   CUtensorMap mk, mv;
   if (int rc = pool_map(ctx, &mk, a.k, a.sk, a, p.page_rows); rc != ADR_OK) return rc;
   if (int rc = pool_map(ctx, &mv, a.v, a.sv, a, p.page_rows); rc != ADR_OK) return rc;
-  const double units = few_units(a, rows, max_rows <= 64);
+  const double units = few_units(a, rows, max_rows <= rows);
   if (a.head_dim == 128)
-    return rows <= 16   ? launch_few_as<128, 1>(ctx, stream, mk, mv, p, units)
-           : rows <= 32 ? launch_few_as<128, 2>(ctx, stream, mk, mv, p, units)
-                        : launch_few_as<128, 4>(ctx, stream, mk, mv, p, units);
-  return rows <= 16   ? launch_few_as<64, 1>(ctx, stream, mk, mv, p, units)
-         : rows <= 32 ? launch_few_as<64, 2>(ctx, stream, mk, mv, p, units)
-                      : launch_few_as<64, 4>(ctx, stream, mk, mv, p, units);
+    return rows <= 16 ? launch_few_as<128, 1>(ctx, stream, mk, mv, p, units) : launch_few_as<128, 2>(ctx, stream, mk, mv, p, units);
+  return rows <= 16 ? launch_few_as<64, 1>(ctx, stream, mk, mv, p, units) : launch_few_as<64, 2>(ctx, stream, mk, mv, p, units);
 }
 
 }  // namespace adr

@@ -755,45 +755,51 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
 }
 
 // Joins a job's parts in their order: a block has 16 rows of a job, a warp one row at a time, HD / 32 columns to a lane.
-constexpr int TJ_ROWS = 16, TJ_THREADS = 128, TL_MAX_SPLITS = 8;
+constexpr int TJ_ROWS = 16, TJ_THREADS = 128, TL_MAX_SPLITS = 32;
 template <int HD>
 __global__ void __launch_bounds__(TJ_THREADS) tiles_join_kernel(const __grid_constant__ TileParams p) {
-  constexpr int PER = HD / 32;
+  constexpr int PER = HD / 32, DEEP = 8;  // columns of a lane, parts whose loads are in flight
   pdl_wait_trigger();
   const int id = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TileJob job = p.job_of[id];
   const int head = id % p.a.n_kv_heads;
   const int n_tok = job.s < p.a.n_seqs ? min(p.tokens_tile, job.span.lq - job.token0) : 0;
   for (int r = blockIdx.y * TJ_ROWS + warp; r < min(n_tok * p.a.group, (int)(blockIdx.y + 1) * TJ_ROWS); r += TJ_THREADS / 32) {
-    float2 x[TL_MAX_SPLITS];
-    float v[TL_MAX_SPLITS][PER];
+    float m = -INFINITY, l = 0.0f, acc[PER] = {};
+    for (int s0 = 0; s0 < p.splits; s0 += DEEP) {
+      float2 x[DEEP];
+      float v[DEEP][PER];
 #pragma unroll
-    for (int i = 0; i < TL_MAX_SPLITS; ++i) {
-      const size_t at = ((size_t)id * p.splits + min(i, p.splits - 1)) * TL_M + r;
-      x[i] = __ldcg(p.part_ml + at);
-      if constexpr (PER == 4) {
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + lane * PER));
-        v[i][0] = y.x, v[i][1] = y.y, v[i][2] = y.z, v[i][3] = y.w;
-      } else {
-        const float2 y = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * HD + lane * PER));
-        v[i][0] = y.x, v[i][1] = y.y;
+      for (int i = 0; i < DEEP; ++i) {
+        const size_t at = ((size_t)id * p.splits + min(s0 + i, p.splits - 1)) * TL_M + r;
+        x[i] = __ldcg(p.part_ml + at);
+        if constexpr (PER == 4) {
+          const float4 y = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + lane * PER));
+          v[i][0] = y.x, v[i][1] = y.y, v[i][2] = y.z, v[i][3] = y.w;
+        } else {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * HD + lane * PER));
+          v[i][0] = y.x, v[i][1] = y.y;
+        }
       }
-    }
-    float top = -INFINITY;
+      float top = m;
 #pragma unroll
-    for (int i = 0; i < TL_MAX_SPLITS; ++i) {
-      if (i >= p.splits) x[i] = make_float2(-INFINITY, 0.0f);
-      top = fmaxf(top, x[i].x);
-    }
-    const float um = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, acc[PER] = {};
+      for (int i = 0; i < DEEP; ++i) {
+        if (s0 + i >= p.splits) x[i] = make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, x[i].x);
+      }
+      const float um = top == -INFINITY ? 0.0f : top, alpha = exp2_fast(m - um);
+      l *= alpha;
 #pragma unroll
-    for (int i = 0; i < TL_MAX_SPLITS; ++i) {
-      if (x[i].x == -INFINITY && x[i].y == 0.0f) continue;  // a part that saw nothing has put down no output
-      const float f = exp2_fast(x[i].x - um);
-      l += x[i].y * f;
+      for (int c = 0; c < PER; ++c) acc[c] *= alpha;
 #pragma unroll
-      for (int c = 0; c < PER; ++c) acc[c] += v[i][c] * f;
+      for (int i = 0; i < DEEP; ++i) {
+        if (x[i].x == -INFINITY && x[i].y == 0.0f) continue;  // a part that saw nothing has put down no output
+        const float f = exp2_fast(x[i].x - um);
+        l += x[i].y * f;
+#pragma unroll
+        for (int c = 0; c < PER; ++c) acc[c] += v[i][c] * f;
+      }
+      m = top;
     }
     const int tok = job.token0 + r / p.a.group, row = job.span.q0 + tok;
     if (row < 0 || row >= p.a.tokens) continue;  // (what another call left, if this one gave up)
