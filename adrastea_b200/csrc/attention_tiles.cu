@@ -25,22 +25,22 @@ namespace adr {
 namespace {
 
 constexpr int TL_M = 128;   // rows of a tile
-constexpr int TL_N = 128;   // keys of a block
 // The workspace: the first bytes are the other kernel's queue, which has to stay as it is.
 constexpr size_t TL_JOBS_AT = 256, TL_PARTS_AT = 16384;
 // Of every eight pairs of probabilities, those that the FMA units compute; the others go to the exponential unit.
 constexpr int BY_FMA = 1;
 
-template <int HD, int NT>
+// N: keys of a block.
+template <int HD, int NT, int N>
 struct TileCfg {
   static constexpr int CH = HD / 64;
-  static constexpr int TILE = 128 * HD * 2;
+  static constexpr int Q_TILE = TL_M * HD * 2, TILE = N * HD * 2;  // bytes of a tile's queries, of a block's keys
   static constexpr int SLOTS = NT == 2 ? 5 : (HD == 128 ? 2 : 4);
   static constexpr int THREADS = NT * 128 + 64;
-  static constexpr uint32_t COLS = NT == 2 ? 512 : 256;
-  static constexpr uint32_t O_COL = NT * 128;
-
-  static constexpr size_t SMEM = 1024 + (size_t)TILE * (NT + SLOTS) + 8 * (5 * NT + 2 * SLOTS) + 64;
+  static constexpr int CTAS = NT == 2 ? 1 : (N == 64 ? 3 : 2);  // to an SM
+  static constexpr uint32_t COLS = NT == 2 ? 512 : (N + HD <= 128 ? 128 : 256);  // of tensor memory: N + HD for a tile
+  static constexpr uint32_t O_COL = NT * N;
+  static constexpr size_t SMEM = 1024 + (size_t)Q_TILE * NT + (size_t)TILE * SLOTS + 8 * (5 * NT + 2 * SLOTS) + 64;
 };
 
 struct TileJob {
@@ -227,15 +227,15 @@ __device__ __forceinline__ bool tile_any(int tile, bool x) {
   return r != 0;
 }
 
-template <int HD, int NT, bool PAGED, bool SPLIT>
-__global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
+template <int HD, int NT, int N, bool PAGED, bool SPLIT>
+__global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N>::CTAS)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TileParams p) {
-  using Cfg = TileCfg<HD, NT>;
-  constexpr int CH = Cfg::CH, SLOTS = Cfg::SLOTS, TILE = Cfg::TILE;
+  using Cfg = TileCfg<HD, NT, N>;
+  constexpr int CH = Cfg::CH, SLOTS = Cfg::SLOTS, TILE = Cfg::TILE, Q_TILE = Cfg::Q_TILE;
   extern __shared__ uint8_t tile_smem[];
   uint8_t* q_sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tile_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* ring = q_sm + NT * TILE;  // K of block 0, V of block 0, K of block 1 ...
+  uint8_t* ring = q_sm + NT * Q_TILE;  // K of block 0, V of block 0, K of block 1 ...
   uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + SLOTS * TILE);  // [NT]
   uint64_t* s_ready = q_full + NT;   // [NT] scores of a tile are complete
   uint64_t* p_ready = s_ready + NT;  // [NT] its probabilities are
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     const int first = token0 + t * p.tokens_tile;
     n_tok[t] = any ? min(p.tokens_tile, max(0, lq - first)) : 0;
     kend[t] = n_tok[t] == 0 ? 0 : p.a.causal ? max(0, lk - lq + first + n_tok[t]) : lk;
-    nb[t] = (kend[t] + TL_N - 1) / TL_N;
+    nb[t] = (kend[t] + N - 1) / N;
     nb_max = max(nb_max, nb[t]);
   }
   int j0 = 0;  // this CTA's first block; blocks are counted from it
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     nb[0] = nb_max = all * (part + 1) / p.splits - j0;
   }
   // keys of a block as the tensor cores take them, in steps of 16
-  auto block_n = [&](int t, int j) { return min(TL_N, (kend[t] - (j0 + j) * TL_N + 15) & ~15); };
+  auto block_n = [&](int t, int j) { return min(N, (kend[t] - (j0 + j) * N + 15) & ~15); };
 
   if (warp == W_TMA) {
     // ------------------------------- producer -------------------------------
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
           if (nb[t] == 0) continue;
           mbar_expect_tx(&q_full[t], (unsigned)(CH * p.tokens_tile * p.a.group * 128));
           for (int c = 0; c < CH; ++c)
-            tma_load_3d(q_sm + t * TILE + c * (TL_M * 128), &map_q, c * 64, head * p.a.group,
+            tma_load_3d(q_sm + t * Q_TILE + c * (TL_M * 128), &map_q, c * 64, head * p.a.group,
                         span.q0 + token0 + t * p.tokens_tile, &q_full[t]);
         }
       }
@@ -352,8 +352,8 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
         if constexpr (PAGED) {
           const int pr = p.page_rows;
-          const int copies = (min(TL_N, lk - j * TL_N) + pr - 1) / pr;
-          const int pos = j * TL_N + lane * pr;
+          const int copies = (min(N, lk - j * N) + pr - 1) / pr;
+          const int pos = j * N + lane * pr;
           int page = 0;
           if (lane < copies) {
             page = __ldg(p.a.block_table + (long long)s_job.s * p.a.max_pages + pos / p.a.page_size);
@@ -368,14 +368,14 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
           __syncwarp();
           if (lane < copies)
             for (int c = 0; c < CH; ++c)
-              tma_load_4d(dst + c * (TL_N * 128) + lane * pr * 128, map, c * 64, head, pos % p.a.page_size, page, &full[st]);
+              tma_load_4d(dst + c * (N * 128) + lane * pr * 128, map, c * 64, head, pos % p.a.page_size, page, &full[st]);
         } else {
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ((unsigned)(i / SLOTS) & 1u) ^ 1u));
           if (!ok) break;
           if (lane == 0) {
             mbar_expect_tx(&full[st], TILE);
             for (int c = 0; c < CH; ++c)
-              tma_load_3d(dst + c * (TL_N * 128), map, c * 64, head, span.q0 + j * TL_N, &full[st]);
+              tma_load_3d(dst + c * (N * 128), map, c * 64, head, span.q0 + j * N, &full[st]);
           }
         }
         issued = i + 1;
@@ -397,10 +397,10 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       const uint32_t leader = elect_one();
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q_lo = desc_lo(smem_u32(q_sm), 16), k_lo = desc_lo(smem_u32(ring), 16),
-                     v_lo = desc_lo(smem_u32(ring), TL_N * 128);
+                     v_lo = desc_lo(smem_u32(ring), N * 128);
       const uint32_t b_q = smem_u32(q_full), b_s = smem_u32(s_ready), b_p = smem_u32(p_ready), b_h = smem_u32(p_half),
                      b_o = smem_u32(o_done), b_full = smem_u32(full), b_empty = smem_u32(empty);
-      constexpr uint32_t CHUNK = TL_N * 128 / 16, SLOT = TILE / 16;  // steps of a descriptor
+      constexpr uint32_t CHUNK = N * 128 / 16, Q_CHUNK = TL_M * 128 / 16, SLOT = TILE / 16;  // steps of a descriptor
       int all_see[NT];  // keys that every row of a tile sees
 #pragma unroll
       for (int t = 0; t < NT; ++t) all_see[t] = p.a.causal ? max(0, lk - lq + token0 + t * p.tokens_tile + 1) : lk;
@@ -417,11 +417,11 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         tc_fence_after_sync();
         if (!ok) return;
         const uint32_t idesc = umma_idesc_f16(block_n(t, j), false), go = leader;
-        const uint32_t qa = q_lo + t * SLOT, ka = k_lo + k_slot(j) * SLOT;
-        umma_ss<false>(tm + t * 128, qa, ka, idesc, go);
+        const uint32_t qa = q_lo + t * (Q_TILE / 16), ka = k_lo + k_slot(j) * SLOT;
+        umma_ss<false>(tm + t * N, qa, ka, idesc, go);
 #pragma unroll
         for (int i = 1; i < CH * 4; ++i)
-          umma_ss<true>(tm + t * 128, qa + (i / 4) * CHUNK + (i % 4) * 2, ka + (i / 4) * CHUNK + (i % 4) * 2, idesc, go);
+          umma_ss<true>(tm + t * N, qa + (i / 4) * Q_CHUNK + (i % 4) * 2, ka + (i / 4) * CHUNK + (i % 4) * 2, idesc, go);
         commit_one(b_s + t * 8, go);
         if (last) commit_one(b_empty + k_slot(j) * 8, go);
       };
@@ -429,19 +429,19 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         wait(b_h + t * 8, (uint32_t)j & 1u);
         tc_fence_after_sync();
         constexpr uint32_t idesc = umma_idesc_f16(HD, true);
-        const uint32_t vd = v_lo + v_slot(j) * SLOT, d = tm + Cfg::O_COL + t * HD, a = tm + t * 128;
-        if ((j0 + j + 1) * TL_N <= all_see[t]) {
+        const uint32_t vd = v_lo + v_slot(j) * SLOT, d = tm + Cfg::O_COL + t * HD, a = tm + t * N;
+        if ((j0 + j + 1) * N <= all_see[t]) {
           if (!ok) return;
           const uint32_t go = leader;
           umma_ts(d, a, vd, idesc, have_o[t], go);
 #pragma unroll
-          for (int i = 1; i < 4; ++i) umma_ts(d, a + i * 8, vd + i * 128, idesc, 1u, go);
+          for (int i = 1; i < N / 32; ++i) umma_ts(d, a + i * 8, vd + i * 128, idesc, 1u, go);
           wait(b_p + t * 8, (uint32_t)j & 1u);
           tc_fence_after_sync();
           if (!ok) return;
           const uint32_t go2 = leader;
 #pragma unroll
-          for (int i = 4; i < 8; ++i) umma_ts(d, a + i * 8, vd + i * 128, idesc, 1u, go2);
+          for (int i = N / 32; i < N / 16; ++i) umma_ts(d, a + i * 8, vd + i * 128, idesc, 1u, go2);
         } else {
           // a block that not every row sees whole: it may be short, or done already
           wait(b_p + t * 8, (uint32_t)j & 1u);
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
     const int warp_most = __reduce_max_sync(0xffffffffu, limit);  // keys that some row of the warp sees
     const int my_end = NT == 2 && t == 1 ? kend[NT - 1] : kend[0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + (uint32_t)(t * 128), o_at = tmem + lanes + Cfg::O_COL + (uint32_t)(t * HD);
+    const uint32_t s_at = tmem + lanes + (uint32_t)(t * N), o_at = tmem + lanes + Cfg::O_COL + (uint32_t)(t * HD);
     // scores in powers of two; the sign of the scale goes into the scores so that the largest product is the maximum
     // (a scale of zero, which would make NaN of what is masked, is as good as one of 1e-30: exp2 is 1 for every score)
     const float scale2 = fmaxf(fabsf(p.a.scale) * 1.4426950408889634f, 1e-30f);
@@ -503,18 +503,18 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
 
     const uint32_t b_s = smem_u32(&s_ready[t]), b_p = smem_u32(&p_ready[t]), b_h = smem_u32(&p_half[t]);
     for (int j = 0; j < my_nb; ++j) {
-      const int key0 = (j0 + j) * TL_N;
-      const bool partly = key0 + TL_N > all_see;  // some row does not see some key of the block
+      const int key0 = (j0 + j) * N;
+      const bool partly = key0 + N > all_see;  // some row does not see some key of the block
       uint8_t* v = ring + ((2 * j + 1) % SLOTS) * TILE;
       bool hand = false;
       // V is waited for, cleared behind the end, and searched for what may not be multiplied by zero.  A thread takes a
       // 16-byte piece of every 128 / (HD / 8)-th row (the swizzle only permutes a row's pieces).
       auto look_at_values = [&] {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[(2 * j + 1) % SLOTS], (unsigned)((2 * j + 1) / SLOTS) & 1u));
-        const int from = max(0, all_see - key0), end = min(TL_N, lk - key0);
-        const int read = min(TL_N, (my_end - key0 + 15) & ~15);  // rows that the tensor cores read
+        const int from = max(0, all_see - key0), end = min(N, lk - key0);
+        const int read = min(N, (my_end - key0 + 15) & ~15);  // rows that the tensor cores read
         constexpr int LPR = HD / 8, STEP = 128 / LPR;
-        uint4* at = reinterpret_cast<uint4*>(v + ((row % LPR) / 8) * (TL_N * 128) + (row % 8) * 16);
+        uint4* at = reinterpret_cast<uint4*>(v + ((row % LPR) / 8) * (N * 128) + (row % 8) * 16);
         uint32_t odd = 0;
         int r = from + row / LPR;
         for (; r + 3 * STEP < min(end, read); r += 4 * STEP) {
@@ -544,19 +544,19 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_s, (unsigned)j & 1u));
       tc_fence_after_sync();
       if (ok && warp_live) {
-        const int chunks = partly ? (min(TL_N, my_end - key0) + 31) / 32 : 4;  // of 32 keys
+        const int chunks = partly ? (min(N, my_end - key0) + 31) / 32 : N / 32;  // of 32 keys
         // the row's maximum
         float mx;
         if (!partly && !negative) {
-          uint32_t s[128];
+          uint32_t s[N];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_x32(s_at + c * 32, s + c * 32);
+          for (int c = 0; c < N / 32; ++c) tmem_ld_x32(s_at + c * 32, s + c * 32);
           tmem_ld_wait();
           float top[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) top[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
 #pragma unroll
-          for (int i = 16; i < 128; i += 2)
+          for (int i = 16; i < N; i += 2)
             top[(i >> 1) & 7] = max3(top[(i >> 1) & 7], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
           mx = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), fmaxf(top[6], top[7]));
         } else {
@@ -618,16 +618,18 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
         // The scores are read a second time, 32 at a time and 32 ahead, rather than kept: that leaves registers for many
         // exponentials at once.  Probabilities are written over scores that have been read.
         if (!partly) {
-          uint32_t s[2][32];
+          constexpr bool AHEAD = N == 128;  // (registers for that are there where few CTAs share an SM)
+          uint32_t s[AHEAD ? 2 : 1][32];
           tmem_ld_x32(s_at, s[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < N / 32; ++c) {
             tmem_ld_wait();
-            if (c < 3) tmem_ld_x32(s_at + (c + 1) * 32, s[(c + 1) & 1]);
+            if (AHEAD && c + 1 < N / 32) tmem_ld_x32(s_at + (c + 1) * 32, s[(c + 1) & 1]);
             uint32_t pk[16];
-            powers(s[c & 1], pk);
+            powers(s[AHEAD ? c & 1 : 0], pk);
             tmem_st_x16(s_at + c * 16, pk);
-            if (c == 1) {
+            if (!AHEAD && c + 1 < N / 32) tmem_ld_x32(s_at + (c + 1) * 32, s[0]);
+            if (c == N / 64 - 1) {
               // the tensor cores may begin
               tmem_wait_st();
               tc_fence_before_sync();
@@ -658,7 +660,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
       if (partly && !early) look_at_values();
       if (hand && ok && warp_live) {
         // this block's product by hand
-        const int end = min(TL_N, my_end - key0);
+        const int end = min(N, my_end - key0);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 8) {
           uint32_t o[8];
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
               const float w = (k & 1) ? __high2float(ph) : __low2float(ph);
               const int r = k0 + k;
               if (key0 + r >= limit) continue;  // (also what lies behind the end)
-              const uint4 x = *reinterpret_cast<const uint4*>(v + (c / 64) * (TL_N * 128) + r * 128 + (((c / 8) ^ r) & 7) * 16);
+              const uint4 x = *reinterpret_cast<const uint4*>(v + (c / 64) * (N * 128) + r * 128 + (((c / 8) ^ r) & 7) * 16);
               const __half2* h = reinterpret_cast<const __half2*>(&x);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -826,25 +828,25 @@ long long most_jobs(const SeqAttention& a, int nt) {
   return std::min<long long>(a.tokens, (a.tokens + a.n_seqs * (per - 1)) / per) * a.n_kv_heads;
 }
 
-template <int HD, int NT, bool PAGED, bool SPLIT>
+template <int HD, int NT, int N, bool PAGED, bool SPLIT>
 int launch_tiles_as(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int min_rows, int splits = 1,
                     uint8_t* workspace = nullptr) {
-  using Cfg = TileCfg<HD, NT>;
-  auto kfn = attention_tiles_kernel<HD, NT, PAGED, SPLIT>;
+  using Cfg = TileCfg<HD, NT, N>;
+  auto kfn = attention_tiles_kernel<HD, NT, N, PAGED, SPLIT>;
   if (int rc = opt_in_smem(ctx, kfn, Cfg::SMEM); rc != ADR_OK) return rc;
   TileParams p = {};
   p.a = a;
   p.tokens_tile = TL_M / a.group;
   p.min_rows = min_rows;
-  p.page_rows = std::min(a.page_size, TL_N);
+  p.page_rows = std::min(a.page_size, N);
   CUtensorMap mq, mk, mv;
   if (int rc = rows_map(ctx, &mq, a.q, a, a.n_heads, a.sq[0], a.sq[1], a.group, p.tokens_tile); rc != ADR_OK) return rc;
   if constexpr (PAGED) {
     if (int rc = pool_map(ctx, &mk, a.k, a.sk, a, p.page_rows); rc != ADR_OK) return rc;
     if (int rc = pool_map(ctx, &mv, a.v, a.sv, a, p.page_rows); rc != ADR_OK) return rc;
   } else {
-    if (int rc = rows_map(ctx, &mk, a.k, a, a.n_kv_heads, a.sk[1], a.sk[2], 1, TL_N); rc != ADR_OK) return rc;
-    if (int rc = rows_map(ctx, &mv, a.v, a, a.n_kv_heads, a.sv[1], a.sv[2], 1, TL_N); rc != ADR_OK) return rc;
+    if (int rc = rows_map(ctx, &mk, a.k, a, a.n_kv_heads, a.sk[1], a.sk[2], 1, N); rc != ADR_OK) return rc;
+    if (int rc = rows_map(ctx, &mv, a.v, a, a.n_kv_heads, a.sv[1], a.sv[2], 1, N); rc != ADR_OK) return rc;
   }
   const long long jobs = most_jobs(a, NT);
   if (jobs > 0x40000000LL) return ADR_ERR_SHAPE;
@@ -890,20 +892,26 @@ int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention
   // tile everywhere (4 x 2048 tokens 135 against 146 us); head_dim 128 of prompts up to 2048 tokens in one (16 x 512: 96
   // against 111 us, 2 x 6000: 576 against 544), over pages, whose copies are many, up to 512 positions only (16 x 200: 42
   // against 43 us, 4 x 512 over 1024: 64 against 59).
+  // Blocks of 64 keys take half the tensor memory where head_dim is 64, and three CTAs fit on an SM: worth it for more short
+  // prompts than two CTAs to an SM would hold (64 x 30 tokens of 32/32 heads 26 against 36 us, 16 x 512: 66 against 72,
+  // 2 x 4096: 237 against 231).
+  const long long jobs = most_jobs(a, 1);
   if (a.block_table == nullptr) {
-    if (a.head_dim == 64) return launch_tiles_as<64, 1, false, false>(ctx, stream, a, min_rows);
-    return max_q <= 2048 ? launch_tiles_as<128, 1, false, false>(ctx, stream, a, min_rows)
-                         : launch_tiles_as<128, 2, false, false>(ctx, stream, a, min_rows);
+    if (a.head_dim == 64)
+      return max_q <= 2048 && jobs > tile_parts(ctx) ? launch_tiles_as<64, 1, 64, false, false>(ctx, stream, a, min_rows)
+                                                     : launch_tiles_as<64, 1, 128, false, false>(ctx, stream, a, min_rows);
+    return max_q <= 2048 ? launch_tiles_as<128, 1, 128, false, false>(ctx, stream, a, min_rows)
+                         : launch_tiles_as<128, 2, 128, false, false>(ctx, stream, a, min_rows);
   }
-  // Few tiles over many keys: the keys of each are shared out among CTAs, at least four blocks to each.
-  const long long jobs = most_jobs(a, 1), blocks = (long long)a.max_pages * a.page_size / TL_N;
-  const int splits = (int)std::min<long long>({tile_parts(ctx) / std::max(jobs, 1LL), blocks / 4, TL_MAX_SPLITS});
+  // Few tiles over many keys: the keys of each are shared out among CTAs, at least 512 to each.
+  const long long keys = (long long)a.max_pages * a.page_size;
+  const int splits = (int)std::min<long long>({tile_parts(ctx) / std::max(jobs, 1LL), keys / 512, TL_MAX_SPLITS});
   if (splits > 1 && (size_t)jobs * sizeof(TileJob) <= TL_PARTS_AT - TL_JOBS_AT)
-    return a.head_dim == 64 ? launch_tiles_as<64, 1, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace)
-                            : launch_tiles_as<128, 1, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace);
-  if (a.head_dim == 64) return launch_tiles_as<64, 1, true, false>(ctx, stream, a, min_rows);
-  return (long long)a.max_pages * a.page_size <= 512 ? launch_tiles_as<128, 1, true, false>(ctx, stream, a, min_rows)
-                                                     : launch_tiles_as<128, 2, true, false>(ctx, stream, a, min_rows);
+    return a.head_dim == 64 ? launch_tiles_as<64, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace)
+                            : launch_tiles_as<128, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace);
+  if (a.head_dim == 64) return launch_tiles_as<64, 1, 128, true, false>(ctx, stream, a, min_rows);
+  return keys <= 512 ? launch_tiles_as<128, 1, 128, true, false>(ctx, stream, a, min_rows)
+                     : launch_tiles_as<128, 2, 128, true, false>(ctx, stream, a, min_rows);
 }
 
 }  // namespace adr
