@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) few_join_kernel(const __grid_con
   const int j = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.a.group;
   const int n = (int)min(p.queue[1], gridDim.x + 1);
   const Segment g = p.begins[j];
+  if (j == 1 && threadIdx.x == 0) p.queue[0] = 0;  // (as the launch before has left it, unless it gave up)
   if (j >= n || g.first == 0) return;  // no item goes across
   const int border = j - 1 - g.place0;
   if (border < 0 || g.place0 < 0 || g.parts < 2 || border > g.parts - 2 || g.place0 + g.parts > n ||

@@ -275,33 +275,46 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
   const int job_id = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
   const int head = job_id % p.a.n_kv_heads;
   if (warp == 0) {
-    // the CTA's tiles: the last ones of a sequence, which see most keys, come first
+    // The CTA's tiles.  The last ones of a sequence, which see most keys, come first, and so do the longest sequences (of
+    // 32 at most: of more there are enough to average out): what starts last should be short.
     int id = job_id / p.a.n_kv_heads;
     const int per = NT * p.tokens_tile;
     TileJob job = {};
     job.s = p.a.n_seqs;
     for (int s0 = 0; s0 < p.a.n_seqs; s0 += 32) {
-      int mine = 0;
+      int mine = 0, keys = 0;
       if (s0 + lane < p.a.n_seqs) {
         const int lq = min(max(__ldg(p.a.cu_q + s0 + lane + 1), 0), p.a.tokens) -
                        min(max(__ldg(p.a.cu_q + s0 + lane), 0), p.a.tokens);
+        keys = PAGED ? __ldg(p.a.kv_len + s0 + lane) : lq;
         if (lq > 0 && (long long)lq * p.a.group >= p.min_rows) mine = (lq + per - 1) / per;
       }
-      int upto = mine;
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += o;
+      int before = 0;  // tiles of sequences that come before the lane's
+      const bool differ = __any_sync(0xffffffffu, lane < p.a.n_seqs && keys != __shfl_sync(0xffffffffu, keys, 0));
+      if (p.a.n_seqs <= 32 && differ) {
+        for (int i = 0; i < p.a.n_seqs; ++i) {
+          const int k = __shfl_sync(0xffffffffu, keys, i), n = __shfl_sync(0xffffffffu, mine, i);
+          if (k > keys || (k == keys && i < lane)) before += n;
+        }
+      } else {
+        int upto = mine;
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += o;
+        }
+        before = upto - mine;
       }
-      const unsigned m = __ballot_sync(0xffffffffu, id < upto);
+      const unsigned m = __ballot_sync(0xffffffffu, id >= before && id < before + mine);
       if (m) {
         const int l = __ffs(m) - 1;
-        const int behind = __shfl_sync(0xffffffffu, upto, l) - 1 - id;  // tiles of the sequence that come later
+        const int behind = __shfl_sync(0xffffffffu, before + mine, l) - 1 - id;  // tiles of the sequence that come later
         job.s = s0 + l;
         job.span = seq_span(p.a.cu_q, p.a.kv_len, job.s, p.a.tokens, p.a.max_pages * p.a.page_size, p.a.status);
         job.token0 = behind * per;
         break;
       }
-      id -= __shfl_sync(0xffffffffu, upto, 31);
+      if (p.a.n_seqs <= 32) break;
+      id -= __shfl_sync(0xffffffffu, before + mine, 31);
     }
     if (lane == 0) {
       s_job = job;
