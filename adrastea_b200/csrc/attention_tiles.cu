@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
         if (lq > 0 && (long long)lq * p.a.group >= p.min_rows) mine = (lq + per - 1) / per;
       }
       int before = 0;  // tiles of sequences that come before the lane's
-      const bool differ = __any_sync(0xffffffffu, lane < p.a.n_seqs && keys != __shfl_sync(0xffffffffu, keys, 0));
+      const int first_keys = __shfl_sync(0xffffffffu, keys, 0);
+      const bool differ = __any_sync(0xffffffffu, lane < p.a.n_seqs && keys != first_keys);
       if (p.a.n_seqs <= 32 && differ) {
         for (int i = 0; i < p.a.n_seqs; ++i) {
           const int k = __shfl_sync(0xffffffffu, keys, i), n = __shfl_sync(0xffffffffu, mine, i);
