@@ -41,7 +41,7 @@ enum {
   ADR_ERR_SHAPE = 2,       /* shape / divisibility / alignment rule violated  */
   ADR_ERR_UNSUPPORTED = 3, /* op the reference has no device code for         */
   ADR_ERR_CUDA = 4,        /* a CUDA call failed; see adr_last_cuda_error     */
-  ADR_ERR_DEVICE = 5,      /* a kernel reported a bounded wait that ran out   */
+  ADR_ERR_DEVICE = 5,      /* a kernel reported a bounded wait that ran out, or a page or length outside its table */
   ADR_ERR_NCCL = 6,
   ADR_ERR_TOO_LARGE = 7    /* operands exceed a fixed built-in buffer (see the entry point) */
 };
@@ -146,7 +146,8 @@ int adr_force_kernel(adr_ctx* ctx, int kernel);
  *               matmul_nt_fp16u8.cu:13-23 (used when block_size >= 64). */
 int adr_set_tunable(adr_ctx* ctx, const char* name, int value);
 /* Synchronises the device and returns ADR_ERR_DEVICE if any kernel launched through this
- * context gave up on a bounded wait (the flag is then cleared), ADR_OK otherwise. */
+ * context gave up on a bounded wait or met a page or length outside its table (the flag is then
+ * cleared), ADR_OK otherwise. */
 int adr_device_status(adr_ctx* ctx);
 /* Kernel family chosen by the most recent successful matmul call. */
 int adr_last_kernel(const adr_ctx* ctx);
@@ -587,7 +588,9 @@ int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, const void*
  * lq of sequence s sees positions 0 .. kv_len[s] - lq + i; a row that sees none becomes zeros.
  * Arithmetic, max_q and rules as in adr_attention_packed; page_size a power of two from 16 to 256.
  * `workspace`: adr_attention_paged_workspace bytes of device memory, 16-byte aligned, zero before its
- * first use; every call leaves it fit for the next.  Calls that overlap in time need one each.
+ * first use and again after a call that ended with ADR_ERR_DEVICE; every other call leaves it fit for
+ * the next.  Calls that overlap in time need one each.  `max_q` should be the largest lq: it chooses
+ * between a kernel of up to 32 rows of a key head and one of tiles of 128.
  */
 size_t adr_attention_paged_workspace(const adr_ctx* ctx, int n_heads, int n_kv_heads, int head_dim);
 int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, const void* q, const void* k_pages,

@@ -214,6 +214,12 @@ PACKED = [  # lens, H, Hk, hd
     ([1] * 70, 4, 2, 128),
     ([1300], 8, 1, 128),
     ([1024, 100], 4, 4, 128),
+    ([30, 1, 77, 64] * 16, 16, 16, 64),   # more tiles than two CTAs to an SM: blocks of 64 keys
+    ([257] * 7, 16, 16, 64),
+    ([200, 129, 65], 128, 128, 64),
+    ([2100, 50], 2, 1, 64),
+    ([2100, 50], 4, 1, 128),              # two tiles to a CTA
+    ([300] * 40, 2, 2, 64),               # more sequences than a warp has lanes
 ]
 
 
@@ -267,13 +273,12 @@ def test_packed_sequences_do_not_touch_each_other(kernels, hd, causal):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("H,Hk", [(2, 2), (8, 1)])
+@pytest.mark.parametrize("H,Hk,n", [(2, 2, 300), (8, 1, 300), (128, 128, 300), (3, 1, 2100)])  # every form of tile
 @pytest.mark.parametrize("at", [0, 20, 150, 299])
 @pytest.mark.parametrize("value", [NAN, float("inf")])
-def test_packed_rows_before_a_bad_token_do_not_see_it(kernels, hd, H, Hk, at, value):
+def test_packed_rows_before_a_bad_token_do_not_see_it(kernels, hd, H, Hk, n, at, value):
     """k and v of one token are not finite: causal rows before it are as if they were, rows from it on see it."""
     g = gen(at + hd)
-    n = 300
     q, k, v = half(g, n, H, hd), half(g, n, Hk, hd), half(g, n, Hk, hd)
     clean_k, clean_v = k.clone(), v.clone()
     v[at, :, 3] = value
@@ -345,6 +350,12 @@ PAGED = [  # new, lens, H, Hk, hd, page, pool layout
     ([2], [9000], 64, 1, 128, 128, "tokens"),
     ([64], [20000], 8, 8, 64, 64, "tokens"),
     ([100, 7], [6000, 6000], 2, 1, 128, 16, "heads"),
+    ([40, 300, 33, 100, 41, 64, 50, 90], [900, 300, 33, 2000, 41, 640, 129, 1000], 16, 16, 128, 16, "tokens"),  # pairs of tiles
+    ([100, 40, 77] * 4, [400, 40, 128] * 4, 16, 16, 128, 32, "pairs"),       # single tiles
+    ([40, 300, 33, 100, 41, 64, 50, 90], [900, 300, 33, 2000, 41, 640, 129, 1000], 16, 16, 64, 64, "heads"),
+    ([3, 8], [3, 2000], 64, 16, 64, 16, "tokens"),                            # 32 rows of a key head
+    ([33], [30000], 1, 1, 128, 256, "tokens"),                                # keys shared out among CTAs
+    ([50, 1, 1, 60], [9000, 9000, 1, 60], 8, 2, 64, 128, "pairs"),
 ]
 
 
@@ -395,11 +406,10 @@ def test_paged_rows_that_see_nothing_are_zeros(kernels, new, lens, hd):
         assert not out[cu[s]:cu[s] + max(0, m - n)].any()
 
 
-@pytest.mark.parametrize("new", [6, 150])
+@pytest.mark.parametrize("new,n,H,Hk", [(6, 400, 8, 2), (20, 300, 1, 1), (150, 400, 8, 2), (150, 3000, 8, 2), (600, 700, 32, 16)])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("value", [NAN, float("inf"), float("-inf")])
-def test_paged_rows_before_a_bad_token_do_not_see_it(kernels, new, hd, value):
-    n, H, Hk = 400, 8, 2
+def test_paged_rows_before_a_bad_token_do_not_see_it(kernels, new, n, H, Hk, hd, value):
     for at in (n - new + 2, n - 1):
         q, P, kv, cu = paged_case([new], [n], H, Hk, hd, 32, "tokens", seed=at)
         k, v = kv[0]
