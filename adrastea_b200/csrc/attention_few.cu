@@ -25,7 +25,8 @@ namespace adr {
 
 namespace {
 
-constexpr int FEW_THREADS = 160;    // four computing warps and the producer
+constexpr int FEW_THREADS = 160;       // four computing warps and the producer
+constexpr int MOST_UNITS = 2000000000;  // units of work that can be counted
 
 constexpr int few_kb(int head_dim) { return 8192 / head_dim; }  // 64 keys of 128 columns, 128 of 64
 
@@ -53,6 +54,7 @@ struct FewParams {
   SeqAttention a;
   int max_rows;  // sequences with more rows of a key head than this are left to another kernel
   int page_rows; // rows of a copy: a page, a stage at most
+  int most_units;  // of all sequences together, by the arguments
   int min_units; // of a CTA, where there are few
   int spare, spare_units;  // small chunks per CTA where a share has at least spare_units units
   float* part_ml;          // [slots][ROWS][2]: two slots to a chunk
@@ -160,14 +162,16 @@ struct FewWork {
   __device__ FewWork(const FewParams& p_, int lane_) : p(p_), lane(lane_), q((p_.a.n_seqs + 31) / 32) {
     int mine = 0;
 #pragma unroll 4
-    for (int i = 0; i < q; ++i) mine += units(lane * q + i);
+    for (int i = 0; i < q; ++i) mine = sum_of(mine, units(lane * q + i));
     upto = scan(mine);
     before = upto - mine;
   }
+  // of two numbers up to MOST_UNITS, staying there (a sequence has fewer units; all of them may not, if spans overlap)
+  __device__ static int sum_of(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)MOST_UNITS); }
   __device__ int scan(int x) const {
     for (int d = 1; d < 32; d <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += o;
+      if (lane >= d) x = sum_of(x, o);
     }
     return x;
   }
@@ -187,6 +191,10 @@ struct FewWork {
   __device__ Share share() const {
     Share r;
     r.total = __shfl_sync(0xffffffffu, upto, 31);
+    if (r.total > p.most_units) {  // more than sequences side by side can have: cu_q is wrong, and nothing is done
+      if (lane == 0) atomicOr(p.a.status, PAGED_BAD);
+      r.total = 0;
+    }
     r.ctas = min((int)gridDim.x, (r.total + p.min_units - 1) / p.min_units);
     r.per = r.ctas ? r.total / r.ctas : 0;
     r.more = r.total - r.per * r.ctas;
@@ -767,6 +775,7 @@ int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, cons
   auto kfn = attention_few_kernel<HD, WM>;
   if (int rc = opt_in_smem(ctx, kfn, Cfg::SMEM); rc != ADR_OK) return rc;
   const int g = few_ctas(ctx);
+  p.most_units = (int)units;
   p.spare = Cfg::SPARE;
   p.part_ml = p.part_o + few_rows<HD, WM>(g) * HD;
   const int ctas = (int)std::min<double>(g, units);
@@ -810,7 +819,7 @@ size_t attention_few_workspace(const adr_ctx* ctx, int head_dim) {
 }
 
 bool attention_few_takes(const SeqAttention& a, int rows, bool one_tile_each) {
-  return few_units(a, rows, one_tile_each) < 2e9;
+  return few_units(a, rows, one_tile_each) < MOST_UNITS;
 }
 
 int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int rows, int max_rows, void* workspace) {

@@ -105,6 +105,7 @@ class PagedCache:
     def extend(self, seqs: list[int], new: list[int]):
         """Room for new[i] more positions of sequence slot seqs[i]; all of them, or MemoryError and none."""
         assert len(set(seqs)) == len(seqs) == len(new) and min(new) >= 0
+        assert all(0 <= s < len(self.length) for s in seqs), "no such sequence slot"
         need = [-(-(self.length[s] + n) // self.page_size) - len(self.pages[s]) for s, n in zip(seqs, new)]
         if any(self.length[s] + n > self.max_pages * self.page_size for s, n in zip(seqs, new)):
             raise MemoryError("a sequence is longer than its row of the block table")
@@ -118,6 +119,7 @@ class PagedCache:
             self.length[s] += n
 
     def release(self, seq: int):
+        assert 0 <= seq < len(self.length), "no such sequence slot"
         self.free += reversed(self.pages[seq])
         self.pages[seq], self.length[seq] = [], 0
 
@@ -440,6 +442,7 @@ class LlamaU8:
     def paged_cache(self, pages: int, page_size: int = 64, max_seqs: int | None = None,
                     max_positions: int | None = None) -> PagedCache:
         """A cache for `extend`; slots for max_batch sequences of max_seq positions unless said otherwise."""
+        assert 16 <= page_size <= 256 and page_size & (page_size - 1) == 0, "a power of two from 16 to 256"
         return PagedCache(self.L, pages, page_size, self.Hl, self.shape.head_dim, max_seqs or self.B,
                           max_positions or self.S, self.device)
 

@@ -509,8 +509,9 @@ int adr_attention_f16(adr_ctx* ctx, adr_stream stream, void* out, const void* q,
  * slot * strides[1] + head * strides[2] + column (elements, 64-bit, not negative).  Query head h
  * belongs to key head h / (n_heads / n_kv_heads).  What the arrays hold is checked on the device:
  * rows are cut to `tokens`, lengths to max_pages * page_size, and a page outside the pool is not
- * written and reads as zeros; each of the last two, and a row at a negative position, also sets the
- * word behind adr_device_status.  A tensor may not overlap one that the same call writes, unless
+ * written and reads as zeros; each of the last two, a row at a negative position, and sequences whose
+ * rows overlap so much that the attention over pages leaves them undone, also set the word behind
+ * adr_device_status.  A tensor may not overlap one that the same call writes, unless
  * its entry says so; two sequences may share pages that neither writes.
  * ------------------------------------------------------------------------ */
 
@@ -575,7 +576,8 @@ int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_out, const vo
  * (scale is not rounded), probabilities are rounded to fp16 for the product with v, the output
  * once.  `max_q`: the longest sequence's rows; it chooses the kernel and does not change what is
  * computed.  head_dim 64 or 128, n_heads a multiple of n_kv_heads and at most 64 times it,
- * pointers 16-byte aligned, strides multiples of 8; else ADR_ERR_SHAPE.
+ * pointers 16-byte aligned, strides of dimensions of more than one element positive multiples of 8;
+ * else ADR_ERR_SHAPE.
  */
 int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, const void* q, const void* k,
                          const void* v, int tokens, int n_seqs, int max_q, int n_heads, int n_kv_heads,

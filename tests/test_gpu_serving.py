@@ -425,6 +425,26 @@ def test_paged_rows_before_a_bad_token_do_not_see_it(kernels, new, n, H, Hk, hd,
         assert not out[first:new, :, 5].isfinite().any()
 
 
+@pytest.mark.parametrize("n,T,positions", [(64, 64, 128), (1025, 2048, 262144)])
+def test_paged_overlapping_sequences_are_left_undone(kernels, n, T, positions):
+    """Every second sequence claims all rows: more work than sequences side by side can have (of the larger case, more
+    than 32 bits count).  Nothing is written and the status word says so; the workspace is fit for the next call."""
+    H, Hk, hd, page = 32, 8, 64, 16
+    q = half(gen(n), T, H, hd)
+    pool = torch.zeros((1, page, Hk, hd), dtype=torch.float16, device="cuda")
+    table = torch.zeros((n, positions // page), dtype=torch.int32, device="cuda")
+    out, ws = torch.full_like(q, 2.0), kernels.attention_paged_workspace(H, Hk, hd)
+    cu, lens = ints([T * (s % 2) for s in range(n + 1)]), ints([positions] * n)
+    kernels.attention_paged(view(out), view(q), pool, pool, table, cu, lens, 8, 0.1, ws)
+    with pytest.raises(AdrError) as e:
+        kernels.device_status()
+    assert e.value.code == 5 and (out == 2.0).all()
+    q, P, kv, cu = paged_case([3], [50], H, Hk, hd, page, "tokens", seed=1)
+    out = torch.empty_like(q)
+    kernels.attention_paged(view(out), view(q), P.k, P.v, P.table, ints(cu), ints([50]), 3, 0.1, ws)
+    assert_close(out[:3], *attend(q[:3], *kv[0], 0.1, 48))
+
+
 @pytest.mark.parametrize("new", [1, 90])
 def test_paged_bad_pages_read_as_zeros(kernels, new):
     """A page outside the pool, a length past the table: zeros and a status, no access."""
