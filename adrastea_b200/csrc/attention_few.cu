@@ -779,26 +779,11 @@ int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, cons
   p.spare = Cfg::SPARE;
   p.part_ml = p.part_o + few_rows<HD, WM>(g) * HD;
   const int ctas = (int)std::min<double>(g, units);
-  if (int rc = launch_whole_sm(ctx, stream, kfn, dim3(ctas), FEW_THREADS, Cfg::SMEM, 1, true, mk, mv, p); rc != ADR_OK)
-    return rc;
+  if (int rc = launch_serving(ctx, stream, kfn, dim3(ctas), FEW_THREADS, Cfg::SMEM, 2, mk, mv, p); rc != ADR_OK) return rc;
   // the borders between the chunks: none where a CTA is all there is, and none inside an item of one block
   const int borders = (int)std::min<double>(ctas * (1 + Cfg::SPARE), units) - 1;
   if (borders < 1 || (long long)p.a.max_pages * p.a.page_size <= Cfg::KB) return ADR_OK;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(borders);
-  cfg.blockDim = dim3(JOIN_THREADS);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, few_join_kernel<HD, Cfg::ROWS>, p);
-  if (e != cudaSuccess) {
-    ctx->last_cuda_error = (int)e;
-    return ADR_ERR_CUDA;
-  }
-  return after_launch(ctx);
+  return launch_serving(ctx, stream, few_join_kernel<HD, Cfg::ROWS>, dim3(borders), JOIN_THREADS, 0, 0, p);
 }
 
 // What the units of the launch can be at most: tiles of `rows` rows, blocks of the longest table row.

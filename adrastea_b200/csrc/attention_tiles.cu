@@ -870,25 +870,10 @@ int launch_tiles_as(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, in
     p.part_ml = reinterpret_cast<float2*>(workspace + TL_PARTS_AT);
     p.part_o = reinterpret_cast<float*>(p.part_ml + jobs * splits * TL_M);
   }
-  if (int rc = launch_whole_sm(ctx, stream, kfn, dim3((unsigned)(jobs * splits)), Cfg::THREADS, Cfg::SMEM, 1, true, mq, mk,
-                               mv, p);
-      rc != ADR_OK || !SPLIT)
+  const dim3 ctas((unsigned)(jobs * splits));
+  if (int rc = launch_serving(ctx, stream, kfn, ctas, Cfg::THREADS, Cfg::SMEM, 2, mq, mk, mv, p); rc != ADR_OK || !SPLIT)
     return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)jobs, TL_M / TJ_ROWS);
-  cfg.blockDim = dim3(TJ_THREADS);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tiles_join_kernel<HD>, p);
-  if (e != cudaSuccess) {
-    ctx->last_cuda_error = (int)e;
-    return ADR_ERR_CUDA;
-  }
-  return after_launch(ctx);
+  return launch_serving(ctx, stream, tiles_join_kernel<HD>, dim3((unsigned)jobs, TL_M / TJ_ROWS), TJ_THREADS, 0, 0, p);
 }
 
 // Parts at once: as many as CTAs that the GPU holds, two to an SM.

@@ -156,10 +156,12 @@ __device__ __forceinline__ void fill_turns(float2 (*turns)[ROPE_MAX_HD / 2], con
   __syncthreads();
 }
 
-// Bound by memory where rows are many (8000 rows of 64 heads of 128: 44 us, 5.9 TB/s).
+// Bound by memory where rows are many (8000 rows of 64 heads of 128: 44 us, 5.9 TB/s).  A block is over in a few chains of
+// loads, so what counts is how many an SM holds: four of the halves (64 registers; at 72 there are three: 4111 rows of 40
+// heads 19.1 against 21.6 us), five of the interleaved (48).
 template <bool HALF, bool VEC, int R>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(__half* out, const __half* in, Strided so, Strided si, int rows,
-                                                            int heads, const int* positions, RopePlan r) {
+__global__ void __launch_bounds__(ROPE_THREADS, HALF ? 4 : 5)
+    rope_kernel(__half* out, const __half* in, Strided so, Strided si, int rows, int heads, const int* positions, RopePlan r) {
   using U = Unit<HALF, VEC>;
   __shared__ float2 turns[R][ROPE_MAX_HD / 2];
   __shared__ int position[R];
@@ -257,26 +259,13 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_append_kernel(const __gr
                         [&](int h) { return vd + h * p.vp.head; });
 }
 
-template <typename... KArgs, typename... Args>
-int launch_rows(adr_ctx* ctx, cudaStream_t stream, void (*kfn)(KArgs...), int blocks, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(ROPE_THREADS);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = ctx->tune_pdl.load() ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kfn, static_cast<KArgs>(args)...);
-  if (e != cudaSuccess) {
-    ctx->last_cuda_error = (int)e;
-    return ADR_ERR_CUDA;
-  }
-  // (as for the other row kernels: with a block per SM and more it fills the GPU)
-  if (blocks >= ctx->sm_count) note_filling_launch(ctx, stream, 4);
-  else ctx->small_before = 1;
-  return after_launch(ctx);
+// (as for the other row kernels: with a block per SM and more it fills the GPU)
+template <typename K, typename... Args>
+int launch_rows(adr_ctx* ctx, cudaStream_t stream, K kfn, int blocks, const Args&... args) {
+  const bool fills = blocks >= ctx->sm_count;
+  if (int rc = launch_serving(ctx, stream, kfn, dim3(blocks), ROPE_THREADS, 0, fills ? 4 : 0, args...); rc != ADR_OK) return rc;
+  if (!fills) ctx->small_before = 1;
+  return ADR_OK;
 }
 
 // From two rows to an SM on they go four to a block (600 rows of 32/8 heads: 5.7 against 8.3 us; 148 rows would take 4.0 either
