@@ -261,14 +261,65 @@ def _stream_handle(stream) -> int:
     return int(stream)
 
 
-@functools.lru_cache(maxsize=4096)
-def _strides2(a: int, b: int):
-    return (C.c_longlong * 2)(a, b)
+_f16 = torch.float16
+
+
+# The serving operators are called once per layer and step, for kernels of a few microseconds.  What follows from the
+# dimensions and strides of a call's arguments is worked out once for all calls with the same ones.
+def _rows(what: str, dims: tuple, strides: tuple, want: tuple):
+    """The token and head strides of a [tokens, heads, head_dim] view."""
+    assert dims == want, f"{what} must be {tuple(want)}, is {tuple(dims)}"
+    assert strides[2] == 1 or dims[2] == 1, f"the columns of {what} must follow one another"
+    return (C.c_longlong * 2)(*strides[:2])
+
+
+def _pool(what: str, dims: tuple, strides: tuple, want: tuple):
+    """The page, slot and head strides of a [pages, page_size, kv_heads, head_dim] tensor."""
+    assert dims == want and strides[3] == 1, f"{what} must be {tuple(want)} with unit column stride"
+    return (C.c_longlong * 3)(*strides[:3])
 
 
 @functools.lru_cache(maxsize=4096)
-def _strides3(a: int, b: int, c: int):
-    return (C.c_longlong * 3)(a, b, c)
+def _rope_plan(out, s_out, x, s_x, positions):
+    T, H, hd = x
+    assert positions == (T,), f"positions must be {(T,)}, is {tuple(positions)}"
+    return T, H, hd, _rows("output", out, s_out, x), _rows("input", x, s_x, x)
+
+
+@functools.lru_cache(maxsize=4096)
+def _packed_plan(out, s_out, q, s_q, k, s_k, v, s_v, cu_q):
+    T, H, hd = q
+    Hk = k[-2]
+    assert len(cu_q) == 1, "cu_q must be [sequences + 1]"
+    return (T, cu_q[0] - 1, H, Hk, hd, _rows("output", out, s_out, q), _rows("q", q, s_q, q),
+            _rows("k", k, s_k, (T, Hk, hd)), _rows("v", v, s_v, (T, Hk, hd)))
+
+
+def _tables(table: tuple, cu_q: tuple, kv_len: tuple):
+    assert len(kv_len) == 1 and len(table) == 2 and table[0] == kv_len[0] and cu_q == (kv_len[0] + 1,), \
+        f"block_table [n, max_pages], cu_q [n + 1] and kv_len [n] are {tuple(table)}, {tuple(cu_q)}, {tuple(kv_len)}"
+
+
+@functools.lru_cache(maxsize=4096)
+def _append_plan(out, s_out, q, s_q, k, s_k, v, s_v, kp, s_kp, vp, s_vp, table, cu_q, kv_len):
+    T, H, hd = q
+    n_pages, page_size, Hk, _ = kp
+    kv = (T, Hk, hd)
+    _tables(table, cu_q, kv_len)
+    return ((T, kv_len[0], H, Hk, hd, _rows("q_out", out, s_out, q), _rows("q", q, s_q, q), _rows("k", k, s_k, kv),
+             _rows("v", v, s_v, kv), _pool("k_pages", kp, s_kp, (n_pages, page_size, Hk, hd)),
+             _pool("v_pages", vp, s_vp, kp)), (table[1], page_size, n_pages))
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_plan(out, s_out, q, s_q, kp, s_kp, vp, s_vp, table, cu_q, kv_len):
+    T, H, hd = q
+    n_pages, page_size, Hk, _ = kp
+    _tables(table, cu_q, kv_len)
+    return ((T, kv_len[0]), (H, Hk, hd, _rows("output", out, s_out, q), _rows("q", q, s_q, q),
+                             _pool("k_pages", kp, s_kp, (n_pages, page_size, Hk, hd)), _pool("v_pages", vp, s_vp, kp)),
+            (table[1], page_size, n_pages))
+
 
 
 class GpuKernels:
@@ -710,33 +761,27 @@ class GpuKernels:
         """The given stream, or the current one of the library's device (whichever device is current)."""
         return _current_stream_of(self.device) if stream is None else _stream_handle(stream)
 
-    def _rows(self, v: TensorView, what: str, dims: tuple):
-        """The token and head strides of a [tokens, heads, head_dim] fp16 view on this device."""
-        lay, base = v.layout, v.base
-        if base.dtype is not torch.float16:
-            raise TypeError(f"{what} must be float16, got {base.dtype}")
-        assert lay.dims == dims, f"{what} must be {dims}, is {lay.dims}"
-        s0, s1, s2 = lay.strides
-        assert s2 == 1 or dims[2] == 1, f"the columns of {what} must follow one another"
-        assert base.get_device() == self.device, f"{what} must be on cuda:{self.device}"
-        return _strides2(s0, s1)
-
-    def _pool(self, t: torch.Tensor, what: str, shape: tuple):
-        """The page, slot and head strides of a [pages, page_size, kv_heads, head_dim] fp16 tensor."""
-        if t.dtype is not torch.float16:
-            raise TypeError(f"{what} must be float16, got {t.dtype}")
-        s0, s1, s2, s3 = t.stride()
-        assert t.shape == shape and s3 == 1, f"{what} must be {tuple(shape)} with unit column stride"
-        assert t.get_device() == self.device, f"{what} must be on cuda:{self.device}"
-        return _strides3(s0, s1, s2)
-
-    def _ints(self, t: torch.Tensor, what: str, dtype=torch.int32):
-        """The address of a contiguous integer array on this device."""
+    def _wrong(self, what: str, t: torch.Tensor, dtype):
         if t.dtype is not dtype:
             raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
-        assert t.is_contiguous() and t.get_device() == self.device, \
-            f"{what} must be contiguous and on cuda:{self.device}"
+        raise AssertionError(f"{what} must be on cuda:{self.device}" +
+                             ("" if t.is_contiguous() else " and contiguous"))
+
+    def _half(self, what: str, t: torch.Tensor) -> int:
+        """The address of an fp16 tensor on this device."""
+        if t.dtype is not _f16 or t.get_device() != self.device:
+            self._wrong(what, t, _f16)
         return t.data_ptr()
+
+    def _ints(self, what: str, t: torch.Tensor, dtype=torch.int32) -> int:
+        """The address of a contiguous integer array on this device."""
+        if t.dtype is not dtype or t.get_device() != self.device or not t.is_contiguous():
+            self._wrong(what, t, dtype)
+        return t.data_ptr()
+
+    def _view(self, what: str, v: TensorView) -> int:
+        """The address of an fp16 view on this device."""
+        return self._half(what, v.base) + 2 * v.offset
 
     def rope_table(self, rotary_dim: int, theta: float, layout: RopeLayout = RopeLayout.Interleaved,
                    scaling: RopeScaling | None = None) -> RopeTable:
@@ -748,51 +793,39 @@ class GpuKernels:
     def rope_f16(self, out: TensorView, input: TensorView, positions: torch.Tensor, table: RopeTable, stream=None):
         """adr_rope_f16: the heads of every row of `input` ([tokens, heads, head_dim]) rotated at
         positions[row] (int32, device).  `out` may be `input`."""
-        dims = T, H, hd = input.layout.dims
-        so, si = self._rows(out, "output", dims), self._rows(input, "input", dims)
-        assert positions.shape == (T,)
-        rc = self._lib.adr_rope_f16(
-            self._ctx, self._stream_of(stream), out.data_ptr(), input.data_ptr(), T, H, hd, so, si,
-            self._ints(positions, "positions"), self._ints(table.turns, "the table", torch.int64), table.rotary_dim,
-            table.amplitude, int(table.layout))
-        self._check(rc)
+        lo, li = out.layout, input.layout
+        T, H, hd, so, si = _rope_plan(lo.dims, lo.strides, li.dims, li.strides, positions.shape)
+        self._check(self._lib.adr_rope_f16(
+            self._ctx, self._stream_of(stream), self._view("output", out), self._view("input", input), T, H, hd, so, si,
+            self._ints("positions", positions), self._ints("the table", table.turns, torch.int64), table.rotary_dim,
+            table.amplitude, table.layout))
 
     def rope_append_paged(self, q_out: TensorView, q: TensorView, k: TensorView, v: TensorView,
                           k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                           cu_q: torch.Tensor, kv_len: torch.Tensor, table: RopeTable, stream=None):
         """adr_rope_append_paged: q of the new tokens rotated into q_out (which may be q), k rotated and
         v copied into the pages [pages, page_size, kv_heads, head_dim] of their sequences."""
-        dims = T, H, hd = q.layout.dims
-        n_pages, page_size, Hk, _ = shape = k_pages.shape
-        n, kv = kv_len.shape[0], (T, Hk, hd)
-        so, sq = self._rows(q_out, "q_out", dims), self._rows(q, "q", dims)
-        sk, sv = self._rows(k, "k", kv), self._rows(v, "v", kv)
-        assert shape[3] == hd
-        skp, svp = self._pool(k_pages, "k_pages", shape), self._pool(v_pages, "v_pages", shape)
-        seqs, max_pages = block_table.shape
-        assert seqs == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
-        rc = self._lib.adr_rope_append_paged(
-            self._ctx, self._stream_of(stream), q_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            k_pages.data_ptr(), v_pages.data_ptr(), T, n, H, Hk, hd, so, sq, sk, sv, skp, svp,
-            self._ints(block_table, "block_table"), self._ints(cu_q, "cu_q"), self._ints(kv_len, "kv_len"),
-            max_pages, page_size, n_pages, self._ints(table.turns, "the table", torch.int64),
-            table.rotary_dim, table.amplitude, int(table.layout))
-        self._check(rc)
+        lo, lq, lk, lv = q_out.layout, q.layout, k.layout, v.layout
+        sizes, pages = _append_plan(lo.dims, lo.strides, lq.dims, lq.strides, lk.dims, lk.strides, lv.dims, lv.strides,
+                                    k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(),
+                                    block_table.shape, cu_q.shape, kv_len.shape)
+        self._check(self._lib.adr_rope_append_paged(
+            self._ctx, self._stream_of(stream), self._view("q_out", q_out), self._view("q", q), self._view("k", k),
+            self._view("v", v), self._half("k_pages", k_pages), self._half("v_pages", v_pages), *sizes,
+            self._ints("block_table", block_table), self._ints("cu_q", cu_q), self._ints("kv_len", kv_len), *pages,
+            self._ints("the table", table.turns, torch.int64), table.rotary_dim, table.amplitude, table.layout))
 
     def attention_packed(self, out: TensorView, q: TensorView, k: TensorView, v: TensorView, cu_q: torch.Tensor,
                          max_q: int, scale: float, mask: MatmulMask = MatmulMask.Causal, stream=None):
         """adr_attention_packed: attention of whole prompts, the rows cu_q[s]..cu_q[s + 1] - 1 of q and out
         ([tokens, heads, head_dim]) and of k and v ([tokens, kv_heads, head_dim]) to a sequence; `max_q`
         is the longest one's rows."""
-        dims = T, H, hd = q.layout.dims
-        Hk = k.layout.dims[-2]
-        so, sq = self._rows(out, "output", dims), self._rows(q, "q", dims)
-        sk, sv = self._rows(k, "k", (T, Hk, hd)), self._rows(v, "v", (T, Hk, hd))
-        assert cu_q.dim() == 1
-        rc = self._lib.adr_attention_packed(
-            self._ctx, self._stream_of(stream), out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), T,
-            cu_q.shape[0] - 1, max_q, H, Hk, hd, so, sq, sk, sv, self._ints(cu_q, "cu_q"), float(scale), int(mask))
-        self._check(rc)
+        lo, lq, lk, lv = out.layout, q.layout, k.layout, v.layout
+        T, n, *sizes = _packed_plan(lo.dims, lo.strides, lq.dims, lq.strides, lk.dims, lk.strides, lv.dims, lv.strides,
+                                    cu_q.shape)
+        self._check(self._lib.adr_attention_packed(
+            self._ctx, self._stream_of(stream), self._view("output", out), self._view("q", q), self._view("k", k),
+            self._view("v", v), T, n, max_q, *sizes, self._ints("cu_q", cu_q), scale, mask))
 
     def attention_paged_workspace(self, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor:
         """A workspace for attention_paged of these heads (zero, as its first use wants it).  Calls that
@@ -805,21 +838,15 @@ class GpuKernels:
                         scale: float, workspace: torch.Tensor, stream=None):
         """adr_attention_paged: the new rows of every sequence over its pages, which hold their own k and
         v already; row i of lq sees the positions up to kv_len - lq + i.  `max_q` is the largest lq."""
-        dims = T, H, hd = q.layout.dims
-        n_pages, page_size, Hk, _ = shape = k_pages.shape
-        n = kv_len.shape[0]
-        so, sq = self._rows(out, "output", dims), self._rows(q, "q", dims)
-        assert shape[3] == hd
-        skp, svp = self._pool(k_pages, "k_pages", shape), self._pool(v_pages, "v_pages", shape)
-        seqs, max_pages = block_table.shape
-        assert seqs == n and cu_q.shape == (n + 1,) and kv_len.dim() == 1
+        lo, lq = out.layout, q.layout
+        rows, sizes, pages = _paged_plan(lo.dims, lo.strides, lq.dims, lq.strides, k_pages.shape, k_pages.stride(),
+                                         v_pages.shape, v_pages.stride(), block_table.shape, cu_q.shape, kv_len.shape)
         assert workspace.is_contiguous() and workspace.get_device() == self.device
-        rc = self._lib.adr_attention_paged(
-            self._ctx, self._stream_of(stream), out.data_ptr(), q.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), T, n, max_q, H, Hk, hd, so, sq, skp, svp, self._ints(block_table, "block_table"),
-            self._ints(cu_q, "cu_q"), self._ints(kv_len, "kv_len"), max_pages, page_size, n_pages,
-            float(scale), workspace.data_ptr(), workspace.numel() * workspace.element_size())
-        self._check(rc)
+        self._check(self._lib.adr_attention_paged(
+            self._ctx, self._stream_of(stream), self._view("output", out), self._view("q", q),
+            self._half("k_pages", k_pages), self._half("v_pages", v_pages), *rows, max_q, *sizes,
+            self._ints("block_table", block_table), self._ints("cu_q", cu_q), self._ints("kv_len", kv_len), *pages,
+            scale, workspace.data_ptr(), workspace.nbytes))
 
     def rms_norm_matmul_nt_fp16u8(self, output: torch.Tensor, lhs: torch.Tensor,
                                   norm_weight: torch.Tensor, eps: float, rhs: torch.Tensor,
