@@ -1,16 +1,18 @@
 // Attention of a few new rows per sequence over a paged cache: single tokens, and a few at a time.
 //
 // The rows of one key head (its query heads times the new tokens, up to 32) share every key and value, so one pass
-// over the cache serves them all: what bounds this kernel is reading the cache once.
-//   * Work is counted in units of 64 keys (of 128 columns; 128 of 64) of one (sequence, key head, tile of rows) and cut into chunks by the lengths
-//     on the device, so the cache of a batch of very different lengths, or of one long sequence, is spread evenly with
-//     no plan from the host.  Every CTA has one chunk of its own, 7/8 of an even share; the rest lies in small chunks
-//     that CTAs take as they get done (SMs do not get equal shares of the memory's bandwidth: with even shares the
-//     slowest of 296 CTAs was done after 94 us where the median one took 77).
+// over the cache serves them all: what bounds this kernel is reading the cache once (64 sequences of 128 to 8192
+// positions, 32/8 heads of 128: 91 us, 512 MB at 5.6 TB/s of 6.55).
+//   * Work is counted in units of one (sequence, key head, tile of rows), 64 keys of 128 columns or 128 of 64, and cut
+//     into one chunk for each CTA by the lengths on the device, so the cache of a batch of very different lengths, or of
+//     one long sequence, is spread evenly with no plan from the host.  (SMs do not get equal shares of the memory's
+//     bandwidth; but to keep an eighth of the work back in small chunks, for CTAs to take as they get done, cost as much
+//     as it gave: 64 sequences 90.7 against 88.4 us, one of 131072 positions 93.4 against 90.1, eight tokens of 64
+//     sequences 130 against 138.)
 //   * The producer warp looks up what comes next and copies pages by TMA into a ring of stages (a unit's keys and values),
 //     across the borders of items.
 //   * Four warps compute: S = Q K^T and O += P V by mma.sync m16n8k16 with the 16 (32) rows as M and a running
-//     maximum and sum.  (tcgen05 wants 64 or 128 rows: at up to 16 live ones the tensor work is 5 % of the time that
+//     maximum and sum.  (tcgen05 wants 64 or 128 rows: at up to 16 live ones the tensor work is 17 % of the time that
 //     the keys take to arrive.  With 64 rows, a row tile to each warp, this kernel took 1.3 to 2.5 times what the tiles of
 //     attention_tiles.cu take.)  With 16 rows the warps share a stage's keys among them, with 32 two by two.
 //   * An item that lies within one chunk is finished there.  Otherwise each part stores its maximum, sum and unscaled
@@ -44,7 +46,6 @@ struct FewCfg {
   static constexpr int SEGS = STAGES + 2;       // descriptors in flight (a segment has at least one stage)
   static constexpr size_t SMEM = (size_t)STAGES * 2 * TILE + MERGE + 4 * 16 * 8 + 16 * STAGES + 8 * SEGS +
                                  SEGS * 48;
-  static constexpr int SPARE = WM == 1 ? 2 : 1;  // small chunks per CTA
   static_assert(WM == 1 || WM == 2, "");
 };
 
@@ -55,11 +56,9 @@ struct FewParams {
   int max_rows;  // sequences with more rows of a key head than this are left to another kernel
   int page_rows; // rows of a copy: a page, a stage at most
   int most_units;  // of all sequences together, by the arguments
-  int min_units; // of a CTA, where there are few
-  int spare, spare_units;  // small chunks per CTA where a share has at least spare_units units
   float* part_ml;          // [slots][ROWS][2]: two slots to a chunk
   float* part_o;           // [slots][ROWS][head_dim]
-  unsigned int* queue;     // small chunks taken so far; then the number of chunks of the call
+  int* chunks;             // their number in this call
   Segment* begins;  // the first segment of every chunk
 };
 
@@ -106,40 +105,13 @@ struct Walk {
   int tiles, blks;
 };
 
-// How the units are cut: the list is divided evenly into `ctas` spans, each of which is a CTA's own chunk and `spare`
-// small ones behind it.  Chunk 0 .. ctas - 1 are the CTAs' own, ctas + c * spare + i the small ones of span c.
+// How the units are cut: the list is divided evenly into `ctas` chunks (the first `more` have one more than `per`).
 struct Share {
-  int total, ctas, spare;
-  int per, more;      // units of a span (the first `more` spans have one more)
-  __device__ int span_begin(int c) const { return c * per + min(c, more); }
-  __device__ int own(int size) const { return spare ? size - size / 8 : size; }
-  __device__ int2 range(int chunk) const {
-    if (chunk < ctas) {
-      const int b = span_begin(chunk);
-      return make_int2(b, b + own(span_begin(chunk + 1) - b));
-    }
-    const int c = (chunk - ctas) / spare, i = chunk - ctas - c * spare;
-    const int b = span_begin(c), e = span_begin(c + 1), first = b + own(e - b), rest = e - first;
-    return make_int2(first + rest * i / spare, first + rest * (i + 1) / spare);
-  }
-  // the place of unit u's chunk in the order of the units: 1 + spare chunks to a span
-  __device__ int place(int u) const {
+  int total, ctas, per, more;
+  __device__ int begin(int c) const { return c * per + min(c, more); }
+  __device__ int chunk_of(int u) const {
     const int big = more * (per + 1);
-    const int c = u < big ? u / (per + 1) : more + (u - big) / per;
-    const int b = span_begin(c), size = span_begin(c + 1) - b, first = own(size);
-    int at = u - b, i = 0;
-    if (at >= first) {
-      const int rest = size - first;
-      at -= first;
-      while (i < spare - 1 && at >= rest * (i + 1) / spare) ++i;
-      ++i;
-    }
-    return c * (1 + spare) + i;
-  }
-  __device__ int place_of(int chunk) const {
-    if (chunk < ctas) return chunk * (1 + spare);
-    const int c = (chunk - ctas) / spare;
-    return c * (1 + spare) + 1 + chunk - ctas - c * spare;
+    return u < big ? u / (per + 1) : more + (u - big) / per;
   }
 };
 
@@ -149,8 +121,8 @@ struct Segment {
   int head, tile;
   int first, last, blks;    // blocks of this run, of the item; blks == 0: there is no more
   int slot;                 // where a part goes (slots are in the order of the units)
-  int place0, parts;        // places of the item's parts
-  int slot0;                // slot of the first one; the others are the first slots of their places
+  int chunk0, parts;        // chunks of the item's parts
+  int slot0;                // slot of the first one; the others are the first slots of their chunks
 };
 static_assert(sizeof(Segment) == 48, "");
 
@@ -195,10 +167,9 @@ struct FewWork {
       if (lane == 0) atomicOr(p.a.status, PAGED_BAD);
       r.total = 0;
     }
-    r.ctas = min((int)gridDim.x, (r.total + p.min_units - 1) / p.min_units);
+    r.ctas = min((int)gridDim.x, r.total);
     r.per = r.ctas ? r.total / r.ctas : 0;
     r.more = r.total - r.per * r.ctas;
-    r.spare = r.per >= max(p.spare_units, 8 * p.spare) ? p.spare : 0;  // (no small chunk may be empty)
     return r;
   }
   __device__ void enter(Walk& w, int s) const {
@@ -265,13 +236,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) few_join_kernel(const __grid_con
   __shared__ float2 part_ml[WARPS];
   pdl_wait_trigger();
   const int j = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.a.group;
-  const int n = (int)min(p.queue[1], gridDim.x + 1);
+  const int n = min(*p.chunks, (int)gridDim.x + 1);
   const Segment g = p.begins[j];
-  if (j == 1 && threadIdx.x == 0) p.queue[0] = 0;  // (as the launch before has left it, unless it gave up)
   if (j >= n || g.first == 0) return;  // no item goes across
-  const int border = j - 1 - g.place0;
-  if (border < 0 || g.place0 < 0 || g.parts < 2 || border > g.parts - 2 || g.place0 + g.parts > n ||
-      g.slot0 >> 1 != g.place0)
+  const int border = j - 1 - g.chunk0;
+  if (g.chunk0 < 0 || border < 0 || g.parts > n || border > g.parts - 2 || g.chunk0 + g.parts > n || g.slot0 >> 1 != g.chunk0)
     return;
   const int live = min(ROWS, g.lq * group - g.tile * ROWS);
   const bool many = g.parts > DEEP;
@@ -287,7 +256,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) few_join_kernel(const __grid_con
 #pragma unroll
       for (int d = 0; d < DEEP; ++d) {
         const int at = j0 + d * step;
-        const size_t row = (size_t)(at == 0 ? g.slot0 : 2 * (g.place0 + min(at, g.parts - 1))) * ROWS + r;
+        const size_t row = (size_t)(at == 0 ? g.slot0 : 2 * (g.chunk0 + min(at, g.parts - 1))) * ROWS + r;
         x[d] = __ldcg(ml + row);
         if constexpr (PER == 4) {
           v[d] = __ldcg(reinterpret_cast<const float4*>(p.part_o + row * HD + lane * PER));
@@ -393,76 +362,64 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       ++seg;
     };
     auto wait_empty = [&] { return ok && __all_sync(0xffffffffu, mbar_wait(&empty[st], (use & 1u) ^ 1u)); };
-    if (blockIdx.x == 0 && lane == 0) p.queue[1] = (unsigned)(share.ctas * (1 + share.spare));
-    for (int chunk = blockIdx.x; chunk < share.ctas * (1 + share.spare);) {
-      const int2 range = share.range(chunk);
-      const int place = share.place_of(chunk);
-      Walk w = {};
-      if (range.x < range.y) w = work.find(range.x);
-      for (int u = range.x; u < range.y && w.tiles != 0 && ok;) {
-        const int last = min(w.blks, w.blk + range.y - u);
-        Segment g;
-        g.q0 = w.span.q0, g.lq = w.span.lq, g.lk = w.span.lk;
-        g.head = w.head, g.tile = w.tile;
-        g.first = w.blk, g.last = last, g.blks = w.blks;
-        // a chunk has at most two parts: one that begins with it, one that begins behind its beginning
-        g.slot = 2 * place + (u == range.x ? 0 : 1);
-        g.place0 = place, g.parts = 1, g.slot0 = g.slot;
-        if (w.blk != 0 || last != w.blks) {
-          const int i0 = u - w.blk;
-          g.place0 = share.place(i0);
-          g.parts = share.place(i0 + w.blks - 1) - g.place0 + 1;
-          if (w.blk != 0) {
-            const int before_i0 = i0 > 0 ? share.place(i0 - 1) : -1;
-            g.slot0 = 2 * g.place0 + (before_i0 == g.place0 ? 1 : 0);
-          }
+    if (blockIdx.x == 0 && lane == 0) *p.chunks = share.ctas;
+    const int chunk = blockIdx.x, begin = share.begin(chunk), end = chunk < share.ctas ? share.begin(chunk + 1) : begin;
+    Walk w = {};
+    if (begin < end) w = work.find(begin);
+    for (int u = begin; u < end && w.tiles != 0 && ok;) {
+      const int last = min(w.blks, w.blk + end - u);
+      Segment g;
+      g.q0 = w.span.q0, g.lq = w.span.lq, g.lk = w.span.lk;
+      g.head = w.head, g.tile = w.tile;
+      g.first = w.blk, g.last = last, g.blks = w.blks;
+      // a chunk has at most two parts: one that begins with it, one that begins behind its beginning
+      g.slot = 2 * chunk + (u == begin ? 0 : 1);
+      g.chunk0 = chunk, g.parts = 1, g.slot0 = g.slot;
+      if (w.blk != 0 || last != w.blks) {
+        const int i0 = u - w.blk;
+        g.chunk0 = share.chunk_of(i0);
+        g.parts = share.chunk_of(i0 + w.blks - 1) - g.chunk0 + 1;
+        if (w.blk != 0) {
+          const int before_i0 = i0 > 0 ? share.chunk_of(i0 - 1) : -1;
+          g.slot0 = 2 * g.chunk0 + (before_i0 == g.chunk0 ? 1 : 0);
         }
-        publish(g);
-        if (u == range.x && lane == 0) p.begins[place] = g;
-        const int* row = p.a.block_table + (long long)w.s * p.a.max_pages;
-        for (int b = w.blk; b < last; ++b) {
-          const int keys = min(Cfg::KB, w.span.lk - b * Cfg::KB);
-          const int copies = (max(keys, 0) + pr - 1) / pr;  // none: a sequence without positions
-          const int pos = b * Cfg::KB + lane * pr;
-          int page = 0;
-          if (lane < copies) {
-            page = __ldg(row + pos / page_size);
-            if (page < 0 || page >= p.a.n_pages) {
-              page = p.a.n_pages;  // outside the map: zeros arrive
-              atomicOr(p.a.status, PAGED_BAD);
-            }
-          }
-          ok = wait_empty();
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&full[st], (unsigned)(copies * pr * HD * 2 * 2));
-          __syncwarp();
-          if (lane < copies) {
-            uint8_t* k_sm = ring + (size_t)st * 2 * Cfg::TILE + lane * pr * 128;
-            const int slot = pos % page_size;
-#pragma unroll
-            for (int c = 0; c < Cfg::CH; ++c) {
-              tma_load_4d(k_sm + c * Cfg::KB * 128, &map_k, c * 64, w.head, slot, page, &full[st]);
-              tma_load_4d(k_sm + Cfg::TILE + c * Cfg::KB * 128, &map_v, c * 64, w.head, slot, page, &full[st]);
-            }
-          }
-          ++issued;
-          if (++st == STAGES) st = 0, ++use;
-        }
-        u += last - w.blk;
-        if (u < range.y) work.next(w);
       }
-      // The next chunk.  Every CTA with a chunk of its own asks until there is none, so that the queue has come round
-      // to zero when all have.
-      if (share.spare == 0) break;
-      unsigned taken = 0;
-      const unsigned n = (unsigned)(share.ctas * share.spare);
-      if (lane == 0) taken = atomicInc(p.queue, n + share.ctas - 1);
-      taken = __shfl_sync(0xffffffffu, taken, 0);
-      if (taken >= n) break;
-      chunk = share.ctas + (int)taken;
+      publish(g);
+      if (u == begin && lane == 0) p.begins[chunk] = g;
+      const int* row = p.a.block_table + (long long)w.s * p.a.max_pages;
+      for (int b = w.blk; b < last; ++b) {
+        const int keys = min(Cfg::KB, w.span.lk - b * Cfg::KB);
+        const int copies = (max(keys, 0) + pr - 1) / pr;  // none: a sequence without positions
+        const int pos = b * Cfg::KB + lane * pr;
+        int page = 0;
+        if (lane < copies) {
+          page = __ldg(row + pos / page_size);
+          if (page < 0 || page >= p.a.n_pages) {
+            page = p.a.n_pages;  // outside the map: zeros arrive
+            atomicOr(p.a.status, PAGED_BAD);
+          }
+        }
+        ok = wait_empty();
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&full[st], (unsigned)(copies * pr * HD * 2 * 2));
+        __syncwarp();
+        if (lane < copies) {
+          uint8_t* k_sm = ring + (size_t)st * 2 * Cfg::TILE + lane * pr * 128;
+          const int slot = pos % page_size;
+#pragma unroll
+          for (int c = 0; c < Cfg::CH; ++c) {
+            tma_load_4d(k_sm + c * Cfg::KB * 128, &map_k, c * 64, w.head, slot, page, &full[st]);
+            tma_load_4d(k_sm + Cfg::TILE + c * Cfg::KB * 128, &map_v, c * 64, w.head, slot, page, &full[st]);
+          }
+        }
+        ++issued;
+        if (++st == STAGES) st = 0, ++use;
+      }
+      u += last - w.blk;
+      if (u < end) work.next(w);
     }
-    Segment end = {};
-    publish(end);
+    const Segment none = {};
+    publish(none);
     // every copy has landed before the CTA may end
     for (int i = max(0, issued - STAGES); i < issued; ++i)
       if (!mbar_wait(&full[i % STAGES], (unsigned)(i / STAGES) & 1u)) ok = false;
@@ -762,11 +719,11 @@ int few_ctas(const adr_ctx* ctx) { return 2 * (ctx->sm_count > 0 ? ctx->sm_count
 template <int HD, int WM>
 constexpr size_t few_rows(size_t ctas) {
   using Cfg = FewCfg<HD, WM>;
-  return 2 * ctas * (1 + Cfg::SPARE) * Cfg::ROWS;
+  return 2 * ctas * Cfg::ROWS;
 }
-// The queue and the number of chunks, then their first segments.
+// The number of chunks, then their first segments.
 constexpr size_t FEW_HEAD = 256;
-size_t few_begins(size_t ctas) { return (3 * ctas * sizeof(Segment) + 255) / 256 * 256; }
+size_t few_begins(size_t ctas) { return (ctas * sizeof(Segment) + 255) / 256 * 256; }
 
 template <int HD, int WM>
 int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, const CUtensorMap& mv, FewParams p,
@@ -776,12 +733,11 @@ int launch_few_as(adr_ctx* ctx, cudaStream_t stream, const CUtensorMap& mk, cons
   if (int rc = opt_in_smem(ctx, kfn, Cfg::SMEM); rc != ADR_OK) return rc;
   const int g = few_ctas(ctx);
   p.most_units = (int)units;
-  p.spare = Cfg::SPARE;
   p.part_ml = p.part_o + few_rows<HD, WM>(g) * HD;
   const int ctas = (int)std::min<double>(g, units);
   if (int rc = launch_serving(ctx, stream, kfn, dim3(ctas), FEW_THREADS, Cfg::SMEM, 2, mk, mv, p); rc != ADR_OK) return rc;
   // the borders between the chunks: none where a CTA is all there is, and none inside an item of one block
-  const int borders = (int)std::min<double>(ctas * (1 + Cfg::SPARE), units) - 1;
+  const int borders = ctas - 1;
   if (borders < 1 || (long long)p.a.max_pages * p.a.page_size <= Cfg::KB) return ADR_OK;
   return launch_serving(ctx, stream, few_join_kernel<HD, Cfg::ROWS>, dim3(borders), JOIN_THREADS, 0, 0, p);
 }
@@ -811,11 +767,9 @@ int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& 
   FewParams p;
   p.a = a;
   p.max_rows = max_rows;
-  p.min_units = std::max(1, ctx->tune_att_cs.load());
-  p.spare_units = 32;
   p.page_rows = std::min(a.page_size, few_kb(a.head_dim));
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  p.queue = reinterpret_cast<unsigned int*>(at);
+  p.chunks = reinterpret_cast<int*>(at);
   p.begins = reinterpret_cast<Segment*>(at + FEW_HEAD);
   p.part_o = reinterpret_cast<float*>(at + FEW_HEAD + few_begins(few_ctas(ctx)));
   CUtensorMap mk, mv;
@@ -823,8 +777,10 @@ int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& 
   if (int rc = pool_map(ctx, &mv, a.v, a.sv, a, p.page_rows); rc != ADR_OK) return rc;
   const double units = few_units(a, rows, max_rows <= rows);
   if (a.head_dim == 128)
-    return rows <= 16 ? launch_few_as<128, 1>(ctx, stream, mk, mv, p, units) : launch_few_as<128, 2>(ctx, stream, mk, mv, p, units);
-  return rows <= 16 ? launch_few_as<64, 1>(ctx, stream, mk, mv, p, units) : launch_few_as<64, 2>(ctx, stream, mk, mv, p, units);
+    return rows <= 16 ? launch_few_as<128, 1>(ctx, stream, mk, mv, p, units)
+                      : launch_few_as<128, 2>(ctx, stream, mk, mv, p, units);
+  return rows <= 16 ? launch_few_as<64, 1>(ctx, stream, mk, mv, p, units)
+                    : launch_few_as<64, 2>(ctx, stream, mk, mv, p, units);
 }
 
 }  // namespace adr

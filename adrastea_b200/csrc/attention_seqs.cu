@@ -135,7 +135,8 @@ extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, c
   p.scale = scale;
   p.status = ctx->d_status;
   const long long rows = (long long)max_q * p.group;
-  if (rows <= FEW_ROWS && attention_few_takes(p, (int)rows, false)) return launch_attention_few(ctx, (cudaStream_t)stream, p, (int)rows, INT_MAX, workspace);
+  if (rows <= FEW_ROWS && attention_few_takes(p, (int)rows, false))
+    return launch_attention_few(ctx, (cudaStream_t)stream, p, (int)rows, INT_MAX, workspace);
   // all sequences of one length: tiles for all; otherwise those of few rows go to the other kernel
   if ((long long)n_seqs * max_q == tokens || !attention_few_takes(p, FEW_ROWS, true))
     return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1, workspace);

@@ -1,16 +1,24 @@
 // Attention of many rows per sequence, causal or not, over rows of a projection or over a paged cache.
 //
 // A tile is 128 rows of one key head: its `group` query heads times 128 / group tokens, token by token, so that the
-// heads that share keys share their loads and a causal tile spans few tokens.  A CTA takes NT = 2 tiles (neighbouring
-// tokens) over the same keys: while the softmax warps of one tile work, the tensor cores work for the other.
-//   * producer: Q once, then K and V in blocks of 128 keys through a ring of shared-memory slots, by TMA (whole boxes
-//     of rows, or page by page), in the 128-byte swizzle;
+// heads that share keys share their loads and a causal tile spans few tokens.  A CTA takes NT tiles over the same keys: with
+// two of them (neighbouring tokens) the tensor cores work for one while the softmax warps of the other work; with one, two
+// or three CTAs to an SM do that for each other (launch_attention_tiles has the choice).
+//   * producer: Q once, then K and V in blocks of N = 128 (64) keys through a ring of shared-memory slots, by TMA (whole
+//     boxes of rows, or page by page), in the 128-byte swizzle;
 //   * S = Q K^T by tcgen05.mma into tensor memory; P = exp2(scale2 (S - m)) written back over S by one thread per row;
 //     O += P V with P from tensor memory and V as it lies in memory (N-major), O staying in tensor memory;
+//   * the product with V begins when half a block's probabilities are there;
 //   * the maximum m that a row is scaled by is moved only when a score passes it by more than 2^8 (P then stays within
 //     fp16's range, and the sums are fp32): the rescaling of O in tensor memory is rare;
 //   * when S of a block is complete, so is the product with V before it (the tensor cores run in order), so the softmax
-//     warps may touch O and no further barrier is needed.
+//     warps may touch O and no further barrier is needed;
+//   * few tiles over many pages: the keys of each are shared out among CTAs, and a second kernel joins the parts.
+// What bounds it: no unit alone.  Two prompts of 8192 tokens, 64/8 heads of 128: 1.9 ms, 1160 TFLOP/s of 1625 in short runs
+// and 2.2 to 2.3 at the power limit, where the clock falls to 1.63 GHz; the tensor cores are busy for half of the time, the
+// exponential unit for 43 %, issue slots for 36 % (2 x 4096 tokens, 32/8 heads), each softmax pass waiting for the product
+// before it.  Of 257 tokens and head_dim 64 (images): 42 us where memory wants 10: a tile's few blocks are one chain of
+// loads, products and softmax, and every third tile has one row.
 // What a causal row does not see must not reach it even if it is infinite or not a number; a probability of zero does
 // not see to that.  Keys are masked by selection.  Values behind the sequence's end are cleared in shared memory; a
 // block of which some rows see only a part is searched, and where a value that some row does not see is not finite the
@@ -25,8 +33,7 @@ namespace adr {
 namespace {
 
 constexpr int TL_M = 128;   // rows of a tile
-// The workspace: the first bytes are the other kernel's queue, which has to stay as it is.
-constexpr size_t TL_JOBS_AT = 256, TL_PARTS_AT = 16384;
+constexpr size_t TL_PARTS_AT = 16384;  // of the workspace: jobs, then parts
 // Of every eight pairs of probabilities, those that the FMA units compute; the others go to the exponential unit.
 constexpr int BY_FMA = 1;
 
@@ -866,7 +873,7 @@ int launch_tiles_as(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, in
   if (jobs > 0x40000000LL) return ADR_ERR_SHAPE;
   p.splits = splits;
   if constexpr (SPLIT) {
-    p.job_of = reinterpret_cast<TileJob*>(workspace + TL_JOBS_AT);
+    p.job_of = reinterpret_cast<TileJob*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(workspace + TL_PARTS_AT);
     p.part_o = reinterpret_cast<float*>(p.part_ml + jobs * splits * TL_M);
   }
@@ -905,7 +912,7 @@ int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention
   // Few tiles over many keys: the keys of each are shared out among CTAs, at least 512 to each.
   const long long keys = (long long)a.max_pages * a.page_size;
   const int splits = (int)std::min<long long>({tile_parts(ctx) / std::max(jobs, 1LL), keys / 512, TL_MAX_SPLITS});
-  if (splits > 1 && (size_t)jobs * sizeof(TileJob) <= TL_PARTS_AT - TL_JOBS_AT)
+  if (splits > 1 && (size_t)jobs * sizeof(TileJob) <= TL_PARTS_AT)
     return a.head_dim == 64 ? launch_tiles_as<64, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace)
                             : launch_tiles_as<128, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace);
   if (a.head_dim == 64) return launch_tiles_as<64, 1, 128, true, false>(ctx, stream, a, min_rows);

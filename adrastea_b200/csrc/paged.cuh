@@ -48,10 +48,10 @@ __device__ __forceinline__ int find_sequence(const int* cu_q, int n_seqs, int t,
   return lo;
 }
 
-// A launch that may begin while the one before it in its stream ends: the kernels here wait for that one's end before they
-// read or write any memory, so it need not be the caller's choice as it is for kernels that fetch weights ahead (in a stream of
-// equal calls: 4111 rows rotated 21.6 against 22.8 us, a token over 131072 keys 98.0 against 99.9).  `fills`: what note_filling_launch wants to know; 0 for a kernel
-// that does not fill the GPU.
+// A launch that may begin while the one before it in its stream ends: the kernels here wait for that one's end before
+// they read or write any memory, so it need not be the caller's choice as it is for kernels that fetch weights ahead (in
+// a stream of equal calls: 4111 rows rotated 21.6 against 22.8 us, a token over 131072 keys 98.0 against 99.9).
+// `fills`: what note_filling_launch wants to know; 0 for a kernel that does not fill the GPU.
 template <typename... KArgs, typename... Args>
 int launch_serving(adr_ctx* ctx, cudaStream_t stream, void (*kfn)(KArgs...), dim3 grid, unsigned threads, size_t smem,
                    int fills, const Args&... args) {

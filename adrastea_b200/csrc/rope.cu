@@ -417,8 +417,11 @@ extern "C" int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_ou
   auto go = [&](auto kfn, int per) { return launch_rows(ctx, (cudaStream_t)stream, kfn, (tokens + per - 1) / per, p); };
   const bool many = vec && many_rows(ctx, tokens), half = layout == ADR_ROPE_HALF;
   if (many)
-    return half ? go(rope_append_kernel<true, true, ROPE_MANY>, ROPE_MANY) : go(rope_append_kernel<false, true, ROPE_MANY>, ROPE_MANY);
+    return half ? go(rope_append_kernel<true, true, ROPE_MANY>, ROPE_MANY)
+                : go(rope_append_kernel<false, true, ROPE_MANY>, ROPE_MANY);
   if (vec)
-    return half ? go(rope_append_kernel<true, true, ROPE_FEW>, ROPE_FEW) : go(rope_append_kernel<false, true, ROPE_FEW>, ROPE_FEW);
-  return half ? go(rope_append_kernel<true, false, ROPE_FEW>, ROPE_FEW) : go(rope_append_kernel<false, false, ROPE_FEW>, ROPE_FEW);
+    return half ? go(rope_append_kernel<true, true, ROPE_FEW>, ROPE_FEW)
+                : go(rope_append_kernel<false, true, ROPE_FEW>, ROPE_FEW);
+  return half ? go(rope_append_kernel<true, false, ROPE_FEW>, ROPE_FEW)
+              : go(rope_append_kernel<false, false, ROPE_FEW>, ROPE_FEW);
 }

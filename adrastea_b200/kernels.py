@@ -828,10 +828,9 @@ class GpuKernels:
             self._view("v", v), T, n, max_q, *sizes, self._ints("cu_q", cu_q), scale, mask))
 
     def attention_paged_workspace(self, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor:
-        """A workspace for attention_paged of these heads (zero, as its first use wants it).  Calls that
-        overlap in time need one each."""
+        """A workspace for attention_paged of these heads.  Calls that overlap in time need one each."""
         need = self._lib.adr_attention_paged_workspace(self._ctx, n_heads, n_kv_heads, head_dim)
-        return torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", self.device))
+        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", self.device))
 
     def attention_paged(self, out: TensorView, q: TensorView, k_pages: torch.Tensor, v_pages: torch.Tensor,
                         block_table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, max_q: int,

@@ -589,9 +589,8 @@ int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, const void*
  * Attention of the new rows over the paged cache, which holds their own k and v already: row i of
  * lq of sequence s sees positions 0 .. kv_len[s] - lq + i; a row that sees none becomes zeros.
  * Arithmetic, max_q and rules as in adr_attention_packed; page_size a power of two from 16 to 256.
- * `workspace`: adr_attention_paged_workspace bytes of device memory, 16-byte aligned, zero before its
- * first use and again after a call that ended with ADR_ERR_DEVICE; every other call leaves it fit for
- * the next.  Calls that overlap in time need one each.  `max_q` should be the largest lq: it chooses
+ * `workspace`: adr_attention_paged_workspace bytes of device memory, 16-byte aligned, whatever they
+ * hold.  Calls that overlap in time need one each.  `max_q` should be the largest lq: it chooses
  * between a kernel of up to 32 rows of a key head and one of tiles of 128.
  */
 size_t adr_attention_paged_workspace(const adr_ctx* ctx, int n_heads, int n_kv_heads, int head_dim);

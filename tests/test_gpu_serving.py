@@ -379,6 +379,7 @@ def test_paged(kernels, new, lens, H, Hk, hd, page, layout, hint):
     out = torch.full_like(q, 3.0)
     ws = kernels.attention_paged_workspace(H, Hk, hd)
     max_q = {"longest": max(new), "one": 1, "many": 4096}[hint]
+    ws.fill_(255)
     for _ in range(2):  # the second call finds the first one's workspace
         out.fill_(3.0)
         kernels.attention_paged(view(out), view(q), P.k, P.v, P.table, ints(cu), ints(lens), max_q, scale, ws)
