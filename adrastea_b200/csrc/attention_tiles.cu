@@ -15,7 +15,7 @@
 //     warps may touch O and no further barrier is needed;
 //   * few tiles over many pages: the keys of each are shared out among CTAs, and a second kernel joins the parts.
 // What bounds it: no unit alone.  Two prompts of 8192 tokens, 64/8 heads of 128: 1.9 ms, 1160 TFLOP/s of 1625 in short runs
-// and 2.2 to 2.3 at the power limit, where the clock falls to 1.63 GHz; the tensor cores are busy for half of the time, the
+// and 2.2 to 2.3 ms at the power limit, where the clock falls to 1.63 GHz; the tensor cores are busy for half of the time, the
 // exponential unit for 43 %, issue slots for 36 % (2 x 4096 tokens, 32/8 heads), each softmax pass waiting for the product
 // before it.  Of 257 tokens and head_dim 64 (images): 42 us where memory wants 10: a tile's few blocks are one chain of
 // loads, products and softmax, and every third tile has one row.
@@ -273,12 +273,9 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
     }
     mbar_fence_init();
   }
+  // (The launch before this one may be anyone's and not have its tensor memory yet: none is held while it is waited for.)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == W_MMA) tmem_alloc(tmem_slot, Cfg::COLS);
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  // (only now: a launch behind this one may not take the tensor memory that this CTA is waiting for)
-  pdl_wait_trigger();
   const int job_id = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
   const int head = job_id % p.a.n_kv_heads;
   if (warp == 0) {
@@ -329,7 +326,11 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
       if (SPLIT && blockIdx.x % p.splits == 0) p.job_of[job_id] = job;
     }
   }
+  tc_fence_before_sync();
   __syncthreads();
+  tc_fence_after_sync();
+  // (only now: a launch behind this one may not take the tensor memory that this CTA is waiting for)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   const SeqSpan span = s_job.span;
   const int lq = span.lq, lk = span.lk, token0 = s_job.token0;
