@@ -28,7 +28,7 @@ inline int pool_map(adr_ctx* ctx, CUtensorMap* map, const __half* base, const lo
   uint64_t strides[3];
   for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (uint64_t)st[i] * 2 : (uint64_t)a.head_dim * 2;
   const uint32_t box[4] = {64u, 1u, (uint32_t)rows, 1u};
-  return tma_get(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  return tma_encode(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Kernels of a few rows per sequence (attention_few.cu): `rows` rows of a key head at most chooses the tile,

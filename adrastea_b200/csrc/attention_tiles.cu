@@ -841,7 +841,7 @@ int rows_map(adr_ctx* ctx, CUtensorMap* map, const __half* base, const SeqAttent
   const uint64_t strides[2] = {n_heads > 1 ? (uint64_t)s_head * 2 : (uint64_t)a.head_dim * 2,
                                a.tokens > 1 ? (uint64_t)s_row * 2 : (uint64_t)a.head_dim * 2};
   const uint32_t box[3] = {64u, (uint32_t)box_heads, (uint32_t)box_rows};
-  return tma_get(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  return tma_encode(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Jobs that there can be at most: each sequence fills up its last one.

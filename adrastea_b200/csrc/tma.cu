@@ -39,6 +39,30 @@ void tma_destroy(adr_ctx* ctx) {
   ctx->tma_cache = nullptr;
 }
 
+int tma_encode(adr_ctx* ctx, CUtensorMap* out, CUtensorMapDataType dtype, int rank, const void* base,
+               const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+               CUtensorMapSwizzle swizzle) {
+  if (!ctx->encode_tiled_fn || rank < 2 || rank > 4) return ADR_ERR_INVALID;
+  cuuint64_t gdim[4] = {1, 1, 1, 1};
+  cuuint64_t gstride[3] = {16, 16, 16};
+  cuuint32_t bdim[4] = {1, 1, 1, 1};
+  cuuint32_t estride[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    gdim[i] = dims[i];
+    bdim[i] = box[i];
+  }
+  for (int i = 0; i + 1 < rank; ++i) gstride[i] = strides_bytes[i];
+  CUresult r = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled_fn)(
+      out, dtype, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstride, bdim, estride,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    ctx->last_cuda_error = 10000 + (int)r;  // CUresult, offset to tell it from a cudaError_t
+    return ADR_ERR_SHAPE;
+  }
+  return ADR_OK;
+}
+
 int tma_get(adr_ctx* ctx, CUtensorMap* out, CUtensorMapDataType dtype, int rank, const void* base,
             const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
             CUtensorMapSwizzle swizzle) {
@@ -61,24 +85,8 @@ int tma_get(adr_ctx* ctx, CUtensorMap* out, CUtensorMapDataType dtype, int rank,
       return ADR_OK;
     }
   }
-  cuuint64_t gdim[4] = {1, 1, 1, 1};
-  cuuint64_t gstride[3] = {16, 16, 16};
-  cuuint32_t bdim[4] = {1, 1, 1, 1};
-  cuuint32_t estride[4] = {1, 1, 1, 1};
-  for (int i = 0; i < rank; ++i) {
-    gdim[i] = dims[i];
-    bdim[i] = box[i];
-  }
-  for (int i = 0; i + 1 < rank; ++i) gstride[i] = strides_bytes[i];
   CUtensorMap m;
-  CUresult r = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled_fn)(
-      &m, dtype, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstride, bdim, estride,
-      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    ctx->last_cuda_error = 10000 + (int)r;  // CUresult, offset to tell it from a cudaError_t
-    return ADR_ERR_SHAPE;
-  }
+  if (int rc = tma_encode(ctx, &m, dtype, rank, base, dims, strides_bytes, box, swizzle); rc != ADR_OK) return rc;
   {
     std::lock_guard<std::mutex> lock(ctx->mu);
     if (cache->maps.size() > 4096) cache->maps.clear();  // bound the cache

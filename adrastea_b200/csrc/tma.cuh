@@ -22,6 +22,11 @@ void tma_destroy(adr_ctx* ctx);
 // A rank-`rank` (2 to 4) tiled map over `base`.  dims[0] is the innermost extent in
 // elements, strides_bytes[i] the byte pitch of dimension i+1, box the tile in elements.
 // Cached in the context by value of all arguments.  Returns ADR_OK or an error code.
+// tma_encode: the same, not cached (for tensors whose addresses and sizes change from call to call, where looking one up
+// takes as long as making it).
+int tma_encode(adr_ctx* ctx, CUtensorMap* out, CUtensorMapDataType dtype, int rank, const void* base,
+               const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+               CUtensorMapSwizzle swizzle);
 int tma_get(adr_ctx* ctx, CUtensorMap* out, CUtensorMapDataType dtype, int rank, const void* base,
             const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
             CUtensorMapSwizzle swizzle);
