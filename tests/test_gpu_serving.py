@@ -426,6 +426,56 @@ def test_paged_rows_before_a_bad_token_do_not_see_it(kernels, new, n, H, Hk, hd,
         assert not out[first:new, :, 5].isfinite().any()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,n,H,Hk", [(1, 900, 8, 2), (7, 900, 4, 1), (90, 900, 4, 1), (90, 5000, 4, 1)])  # every kernel
+def test_paged_large_scores(kernels, new, n, H, Hk, hd):
+    """Maxima that grow and fall along the keys by hundreds, equal ones; a negative scale and zero."""
+    for kind in ("grow", "fall", "equal", "negative", "zero"):
+        q, P, kv, cu = paged_case([new], [n], H, Hk, hd, 32, "tokens", seed=7)
+        k, v = kv[0]
+        ramp = torch.linspace(-4, 4, n, device="cuda")[:, None, None]
+        if kind in ("grow", "fall"):
+            q = torch.ones_like(q)
+            k = ((ramp if kind == "grow" else -ramp) + 0.1 * k.float()).half()
+        if kind == "equal":
+            k = k[:1].expand(n, Hk, hd).contiguous()
+        P.put(0, 0, k, v)
+        scale = {"negative": -0.2, "zero": 0.0}.get(kind, 0.7)
+        out, ws = torch.empty_like(q), kernels.attention_paged_workspace(H, Hk, hd)
+        kernels.attention_paged(view(out), view(q), P.k, P.v, P.table, ints(cu), ints([n]), new, scale, ws)
+        assert_close(out[:new], *attend(q[:new], k, v, scale, n - new + 1), kind)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_many_sequences(kernels, new):
+    """More sequences than a warp looks up at once, twice over: appended, attended over pages, and packed."""
+    S, H, Hk, hd, page = 1500, 2, 1, 64, 16
+    lens = [new + (i * 7) % 40 for i in range(S)]
+    q, P, kv, cu = paged_case([new] * S, lens, H, Hk, hd, page, "tokens")
+    rope = kernels.rope_table(hd, 10000.0)
+    pos = torch.tensor([n - new + i for n in lens for i in range(new)], device="cuda")
+    g = gen(3)
+    k, v = half(g, cu[-1], Hk, hd), half(g, cu[-1], Hk, hd)
+    turned_q, turned_k, out = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q)
+    at = pos.int()
+    kernels.rope_f16(view(turned_q[:cu[-1]]), view(q[:cu[-1]]), at, rope)
+    kernels.rope_f16(view(turned_k), view(k), at, rope)
+    rows = torch.empty_like(q)
+    kernels.rope_append_paged(view(rows[:cu[-1]]), view(q[:cu[-1]]), view(k), view(v), P.k, P.v, P.table, ints(cu), ints(lens),
+                              rope)
+    assert torch.equal(rows[:cu[-1]], turned_q[:cu[-1]])
+    ws = kernels.attention_paged_workspace(H, Hk, hd)
+    kernels.attention_paged(view(out), view(rows), P.k, P.v, P.table, ints(cu), ints(lens), new, 0.1, ws)
+    packed = torch.empty_like(rows[:cu[-1]])
+    kernels.attention_packed(view(packed), view(rows[:cu[-1]]), view(turned_k), view(v), ints(cu), new, 0.1)
+    kernels.device_status()
+    for s in range(0, S, 7):
+        mine = slice(cu[s], cu[s + 1])
+        keys, values = (torch.cat([old[:lens[s] - new], fresh[mine]]) for old, fresh in zip(kv[s], (turned_k, v)))
+        assert_close(out[mine], *attend(rows[mine], keys, values, 0.1, lens[s] - new + 1), s)
+        assert_close(packed[mine], *attend(rows[mine], turned_k[mine], v[mine], 0.1, 1), s)
+
+
 @pytest.mark.parametrize("n,T,positions", [(64, 64, 128), (1025, 2048, 262144)])
 def test_paged_overlapping_sequences_are_left_undone(kernels, n, T, positions):
     """Every second sequence claims all rows: more work than sequences side by side can have (of the larger case, more
