@@ -3,9 +3,10 @@
 // A tile is 128 rows of one key head: its `group` query heads times 128 / group tokens, token by token, so that the
 // heads that share keys share their loads and a causal tile spans few tokens.  A CTA takes NT tiles over the same keys: with
 // two of them (neighbouring tokens) the tensor cores work for one while the softmax warps of the other work; with one, two
-// or three CTAs to an SM do that for each other (launch_attention_tiles has the choice).
+// or four CTAs to an SM do that for each other (launch_attention_tiles has the choice).
 //   * producer: Q once, then K and V in blocks of N = 128 (64) keys through a ring of shared-memory slots, by TMA (whole
-//     boxes of rows, or page by page), in the 128-byte swizzle;
+//     boxes of rows, or page by page), in the 128-byte swizzle; with N = 64 the tensor-core warp does that too (160
+//     threads: four CTAs to an SM have 96 registers a thread, of 192 they would have 80);
 //   * S = Q K^T by tcgen05.mma into tensor memory; P = exp2(scale2 (S - m)) written back over S by one thread per row;
 //     O += P V with P from tensor memory and V as it lies in memory (N-major), O staying in tensor memory;
 //   * the product with V begins when half a block's probabilities are there;
@@ -17,8 +18,8 @@
 // What bounds it: no unit alone.  Two prompts of 8192 tokens, 64/8 heads of 128: 1.9 ms, 1160 TFLOP/s of 1625 in short runs
 // and 2.2 to 2.3 ms at the power limit, where the clock falls to 1.63 GHz; the tensor cores are busy for half of the time, the
 // exponential unit for 43 %, issue slots for 36 % (2 x 4096 tokens, 32/8 heads), each softmax pass waiting for the product
-// before it.  Of 257 tokens and head_dim 64 (images): 42 us where memory wants 10: a tile's few blocks are one chain of
-// loads, products and softmax, and every third tile has one row.
+// before it.  Of 257 tokens and head_dim 64 (images): 38 us where memory wants 10: each CTA begins and ends in about 5
+// us of latency, a third of which the other three hide, and every third tile has one row.
 // What a causal row does not see must not reach it even if it is infinite or not a number; a probability of zero does
 // not see to that.  Keys are masked by selection.  Values behind the sequence's end are cleared in shared memory; a
 // block of which some rows see only a part is searched, and where a value that some row does not see is not finite the
@@ -43,8 +44,9 @@ struct TileCfg {
   static constexpr int CH = HD / 64;
   static constexpr int Q_TILE = TL_M * HD * 2, TILE = N * HD * 2;  // bytes of a tile's queries, of a block's keys
   static constexpr int SLOTS = NT == 2 ? 5 : (HD == 128 ? 2 : 4);
-  static constexpr int THREADS = NT * 128 + 64;
-  static constexpr int CTAS = NT == 2 ? 1 : (N == 64 ? 3 : 2);  // to an SM
+  static constexpr bool ONE = N == 64;  // one warp loads and issues the products
+  static constexpr int THREADS = NT * 128 + (ONE ? 32 : 64);
+  static constexpr int CTAS = NT == 2 ? 1 : (N == 64 ? 4 : 2);  // to an SM
   static constexpr uint32_t COLS = NT == 2 ? 512 : (N + HD <= 128 ? 128 : 256);  // of tensor memory: N + HD for a tile
   static constexpr uint32_t O_COL = NT * N;
   static constexpr size_t SMEM = 1024 + (size_t)Q_TILE * NT + (size_t)TILE * SLOTS + 8 * (5 * NT + 2 * SLOTS) + 64;
@@ -255,7 +257,8 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
   __shared__ TileJob s_job;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int W_MMA = NT * 4, W_TMA = NT * 4 + 1;
+  constexpr bool ONE = Cfg::ONE;
+  constexpr int W_MMA = NT * 4, W_TMA = NT * 4 + (ONE ? 0 : 1);
   if (warp == W_TMA && lane == 0) {
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_k);
@@ -275,6 +278,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
   }
   // (The launch before this one may be anyone's and not have its tensor memory yet: none is held while it is waited for.)
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  __syncwarp();
   if (warp == W_MMA) tmem_alloc(tmem_slot, Cfg::COLS);
   const int job_id = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
   const int head = job_id % p.a.n_kv_heads;
@@ -354,7 +358,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
   // keys of a block as the tensor cores take them, in steps of 16
   auto block_n = [&](int t, int j) { return min(N, (kend[t] - (j0 + j) * N + 15) & ~15); };
 
-  if (warp == W_TMA) {
+  if (!ONE && warp == W_TMA) {
     // ------------------------------- producer -------------------------------
     bool ok = true;
     if (nb_max > 0) {
@@ -479,7 +483,30 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
         if (j == nb[t] - 1) commit_one(b_o + t * 8, go);
       };
       // tile 1 sees at least what tile 0 sees, so a block's last user is tile 1 where it takes part
-      auto last = [&](int t, int j) { return NT == 1 || t == 1 || j >= nb[NT - 1]; };
+      auto last = [&](int t, int j) { return !ONE && (NT == 1 || t == 1 || j >= nb[NT - 1]); };
+      // Without a producer: copy i of K of block 0, V of block 0, K of block 1 ..., into a slot that is free.
+      int issued = 0;
+      auto load = [&](int i) {
+        if (!ok || i >= 2 * nb_max) return;
+        if (leader) {
+          mbar_expect_tx(&full[i % SLOTS], TILE);
+          for (int c = 0; c < CH; ++c)
+            tma_load_3d(ring + (i % SLOTS) * TILE + c * (N * 128), (i & 1) ? &map_v : &map_k, c * 64, head,
+                        span.q0 + (i >> 1) * N, &full[i % SLOTS]);
+        }
+        issued = i + 1;
+        __syncwarp();
+      };
+      if constexpr (ONE) {
+        static_assert(NT == 1 && !PAGED && !SPLIT && SLOTS == 4, "");
+        if (leader) {
+          mbar_expect_tx(q_full, (unsigned)(CH * p.tokens_tile * p.a.group * 128));
+          for (int c = 0; c < CH; ++c)
+            tma_load_3d(q_sm + c * (TL_M * 128), &map_q, c * 64, head * p.a.group, span.q0 + token0, q_full);
+        }
+        __syncwarp();
+        for (int i = 0; i < SLOTS; ++i) load(i);
+      }
       wait_k(0);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -496,6 +523,19 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
           if (j < nb[t]) output(t, j, last(t, j));
           if (j + 1 < nb[t]) scores(t, j + 1, last(t, j + 1));
         }
+        if constexpr (ONE) {
+          // The probabilities of block j are there, so its scores are, and what was issued before them: the product with V of
+          // block j - 1.  Their slots are free.
+          if (j > 0) load(2 * j + 3);
+          load(2 * j + 4);
+        }
+      }
+      if constexpr (ONE) {
+        // every copy has landed before the CTA may end
+        bool landed = mbar_wait(q_full, 0);
+        for (int i = max(0, issued - SLOTS); i < issued; ++i)
+          if (!mbar_wait(&full[i % SLOTS], (unsigned)(i / SLOTS) & 1u)) landed = false;
+        ok = __all_sync(0xffffffffu, ok && landed);
       }
       if (!ok && lane == 0) atomicOr(p.a.status, 1u << 24);
     }
@@ -899,14 +939,16 @@ int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention
   // tile everywhere (4 x 2048 tokens 135 against 146 us); head_dim 128 of prompts up to 2048 tokens in one (16 x 512: 96
   // against 111 us, 2 x 6000: 576 against 544), over pages, whose copies are many, up to 512 positions only (16 x 200: 42
   // against 43 us, 4 x 512 over 1024: 64 against 59).
-  // Blocks of 64 keys take half the tensor memory where head_dim is 64, and three CTAs fit on an SM: worth it for more short
-  // prompts than two CTAs to an SM would hold (64 x 30 tokens of 32/32 heads 26 against 36 us, 16 x 512: 66 against 72,
-  // 2 x 4096: 237 against 231).
+  // Blocks of 64 keys take half the tensor memory where head_dim is 64, and without a warp for the copies four CTAs fit on an
+  // SM.  Worth it where there are enough tiles for all of them, of long causal ones, which differ, twice as many: 16/16 heads,
+  // causal: 4 x 2048 tokens (1024 tiles) 93 against 78 us, 16 x 512 (1024) 39 against 39; all keys seen: 16 x 512 36 against
+  // 42, 4 x 2048 107 against 120; 32/32 heads, causal: 1 x 2048 (512 tiles) 46 against 42, 2 x 8192 (4096) 749 against 813.
   const long long jobs = most_jobs(a, 1);
   if (a.block_table == nullptr) {
     if (a.head_dim == 64)
-      return max_q <= 2048 && jobs > tile_parts(ctx) ? launch_tiles_as<64, 1, 64, false, false>(ctx, stream, a, min_rows)
-                                                     : launch_tiles_as<64, 1, 128, false, false>(ctx, stream, a, min_rows);
+      return jobs > (a.causal && max_q > 512 ? 4 : 2) * tile_parts(ctx)
+                 ? launch_tiles_as<64, 1, 64, false, false>(ctx, stream, a, min_rows)
+                 : launch_tiles_as<64, 1, 128, false, false>(ctx, stream, a, min_rows);
     return max_q <= 2048 ? launch_tiles_as<128, 1, 128, false, false>(ctx, stream, a, min_rows)
                          : launch_tiles_as<128, 2, 128, false, false>(ctx, stream, a, min_rows);
   }

@@ -220,6 +220,8 @@ PACKED = [  # lens, H, Hk, hd
     ([2100, 50], 2, 1, 64),
     ([2100, 50], 4, 1, 128),              # two tiles to a CTA
     ([300] * 40, 2, 2, 64),               # more sequences than a warp has lanes
+    ([129, 130, 131, 132, 133, 257], 2, 1, 64),             # a few keys behind a full block
+    ([65, 130, 195, 260, 69, 129, 2, 64] * 8, 16, 16, 64),
 ]
 
 
@@ -273,7 +275,7 @@ def test_packed_sequences_do_not_touch_each_other(kernels, hd, causal):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("H,Hk,n", [(2, 2, 300), (8, 1, 300), (128, 128, 300), (3, 1, 2100)])  # every form of tile
+@pytest.mark.parametrize("H,Hk,n", [(2, 2, 300), (8, 1, 300), (256, 256, 300), (3, 1, 2100)])  # every form of tile
 @pytest.mark.parametrize("at", [0, 20, 150, 299])
 @pytest.mark.parametrize("value", [NAN, float("inf")])
 def test_packed_rows_before_a_bad_token_do_not_see_it(kernels, hd, H, Hk, n, at, value):
@@ -299,9 +301,10 @@ def test_packed_rows_before_a_bad_token_do_not_see_it(kernels, hd, H, Hk, n, at,
 
 
 @pytest.mark.parametrize("hd", [64, 128])
-def test_packed_large_scores(kernels, hd):
+@pytest.mark.parametrize("H", [2, 256])
+def test_packed_large_scores(kernels, H, hd):
     """Maxima that grow along the keys by hundreds, falling ones, and equal ones; a negative scale and zero."""
-    n, H = 520, 2
+    n = 520
     g = gen(1)
     for kind in ("grow", "fall", "equal", "negative", "zero"):
         q, k, v = half(g, n, H, hd), half(g, n, H, hd), half(g, n, H, hd)
@@ -315,6 +318,40 @@ def test_packed_large_scores(kernels, hd):
         out = torch.empty_like(q)
         kernels.attention_packed(view(out), view(q), view(k), view(v), ints([0, n]), n, scale)
         assert_close(out, *attend(q, k, v, scale, 1), kind)
+
+
+@pytest.mark.parametrize("n,S", [(258, 1), (260, 20)])
+def test_packed_last_keys_of_every_size(kernels, n, S):
+    """The keys behind the last full block have the largest scores, the smallest, or equal ones; a negative scale, zero; one of
+    them, or its value, is not finite, which every row sees."""
+    H, hd = 16, 64
+    g = gen(n)
+    for kind in ("largest", "smallest", "equal", "negative", "zero", "key", "value"):
+        q, k, v = (half(g, S, n, H, hd) for _ in "qkv")
+        if kind in ("largest", "smallest"):
+            q = torch.ones_like(q)
+            k[:, 256:] = 5.0 if kind == "largest" else -5.0
+        if kind == "equal":
+            k = k[:, :1].expand(S, n, H, hd).contiguous()
+        if kind == "key":
+            k[:, n - 1, 0] = NAN
+        if kind == "value":
+            v[:, n - 1, 0, 3] = float("inf")
+        scale = {"negative": -0.2, "zero": 0.0}.get(kind, 0.3)
+        out = torch.empty_like(q)
+        kernels.attention_packed(view(out.view(S * n, H, hd)), view(q.view(S * n, H, hd)), view(k.view(S * n, H, hd)),
+                                 view(v.view(S * n, H, hd)), ints([n * s for s in range(S + 1)]), n, scale, MatmulMask.None_)
+        if kind == "key":
+            assert out[:, :, 0].isnan().all()
+            out, q, k, v = (t[:, :, 1:] for t in (out, q, k, v))
+        if kind == "value":
+            assert (out[:, :, 0, 3] == float("inf")).all()
+            v[:, n - 1, 0, 3] = out[:, :, 0, 3] = 0.0
+        for s in range(0, S, 5):
+            want, tol = attend(q[s], k[s], v[s], scale, None)
+            if kind == "value":
+                want[:, 0, 3] = 0.0
+            assert_close(out[s], want, tol, (kind, s))
 
 
 def test_packed_wrong_spans_stay_inside(kernels):
