@@ -14,6 +14,11 @@ namespace {
 // in tiles, 32 x 1000: 46 against 40; from 40 rows on the tiles are ahead nearly everywhere, 32 x 1000: 160 against 143.)
 constexpr int FEW_ROWS = 32;
 
+// Keys of a tile's part up to which a second kernel for the sequences of few rows costs more than their tiles (6 sequences of
+// up to 100 tokens over up to 4096 positions, 32/8 heads: 43 against 56 us; a single token's tile over more would be what all
+// others wait for).
+constexpr int ALONE_KEYS = 4096;
+
 // The strides of n dimensions of the given extents: not negative, and 16-byte steps where a dimension has more
 // than one element.
 int check_steps(const void* base, const long long* strides, int n, const int* extents) {
@@ -137,8 +142,11 @@ extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, c
   const long long rows = (long long)max_q * p.group;
   if (rows <= FEW_ROWS && attention_few_takes(p, (int)rows, false))
     return launch_attention_few(ctx, (cudaStream_t)stream, p, (int)rows, INT_MAX, workspace);
-  // all sequences of one length: tiles for all; otherwise those of few rows go to the other kernel
-  if ((long long)n_seqs * max_q == tokens || !attention_few_takes(p, FEW_ROWS, true))
+  // All sequences of one length, or all tiles on the GPU at once with at most ALONE_KEYS keys each: tiles for all.  Otherwise
+  // those of few rows go to the other kernel.
+  const int splits = attention_tiles_splits(ctx, p);
+  const bool at_once = splits > 1 && (long long)max_pages * page_size <= (long long)splits * ALONE_KEYS;
+  if ((long long)n_seqs * max_q == tokens || at_once || !attention_few_takes(p, FEW_ROWS, true))
     return launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, 1, workspace);
   if (int rc = launch_attention_tiles(ctx, (cudaStream_t)stream, p, max_q, FEW_ROWS + 1, workspace); rc != ADR_OK)
     return rc;

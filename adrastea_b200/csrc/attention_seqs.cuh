@@ -41,6 +41,8 @@ int launch_attention_few(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& 
 
 // Tiles of many rows (attention_tiles.cu): sequences with fewer than min_rows rows of a key head are passed over.  The
 // workspace is used over pages only.
+// attention_tiles_splits: how many CTAs share a tile's keys over pages; more than one: all tiles are on the GPU at once.
+int attention_tiles_splits(const adr_ctx* ctx, const SeqAttention& a);
 size_t attention_tiles_workspace(const adr_ctx* ctx, int head_dim);
 int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int max_q, int min_rows,
                            void* workspace);

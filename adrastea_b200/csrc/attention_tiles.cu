@@ -933,6 +933,15 @@ size_t attention_tiles_workspace(const adr_ctx* ctx, int head_dim) {
   return TL_PARTS_AT + (size_t)tile_parts(ctx) * TL_M * (head_dim + 2) * sizeof(float);
 }
 
+int attention_tiles_splits(const adr_ctx* ctx, const SeqAttention& a) {
+  // Few tiles over many keys: the keys of each are shared out among CTAs, at least 256 to each (220 tokens over 1423 positions,
+  // 16/16 heads: 23.8 us, of 512 to each 27.2).
+  const long long jobs = most_jobs(a, 1), keys = (long long)a.max_pages * a.page_size;
+  if ((size_t)jobs * sizeof(TileJob) > TL_PARTS_AT) return 1;
+  const long long splits = std::min<long long>({tile_parts(ctx) / std::max(jobs, 1LL), keys / 256, TL_MAX_SPLITS});
+  return (int)std::max(splits, 1LL);
+}
+
 int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int max_q, int min_rows, void* workspace) {
   // One tile to a CTA and two CTAs to an SM, or two tiles that share their keys.  The former hides one CTA's start and
   // end behind the other's work, the latter halves what is loaded; measured on 32/32 and 32/8 heads: head_dim 64 in one
@@ -943,8 +952,8 @@ int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention
   // SM.  Worth it where there are enough tiles for all of them, of long causal ones, which differ, twice as many: 16/16 heads,
   // causal: 4 x 2048 tokens (1024 tiles) 93 against 78 us, 16 x 512 (1024) 39 against 39; all keys seen: 16 x 512 36 against
   // 42, 4 x 2048 107 against 120; 32/32 heads, causal: 1 x 2048 (512 tiles) 46 against 42, 2 x 8192 (4096) 749 against 813.
-  const long long jobs = most_jobs(a, 1);
   if (a.block_table == nullptr) {
+    const long long jobs = most_jobs(a, 1);
     if (a.head_dim == 64)
       return jobs > (a.causal && max_q > 512 ? 4 : 2) * tile_parts(ctx)
                  ? launch_tiles_as<64, 1, 64, false, false>(ctx, stream, a, min_rows)
@@ -952,15 +961,14 @@ int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention
     return max_q <= 2048 ? launch_tiles_as<128, 1, 128, false, false>(ctx, stream, a, min_rows)
                          : launch_tiles_as<128, 2, 128, false, false>(ctx, stream, a, min_rows);
   }
-  // Few tiles over many keys: the keys of each are shared out among CTAs, at least 512 to each.
-  const long long keys = (long long)a.max_pages * a.page_size;
-  const int splits = (int)std::min<long long>({tile_parts(ctx) / std::max(jobs, 1LL), keys / 512, TL_MAX_SPLITS});
-  if (splits > 1 && (size_t)jobs * sizeof(TileJob) <= TL_PARTS_AT)
+  const int splits = attention_tiles_splits(ctx, a);
+  if (splits > 1)
     return a.head_dim == 64 ? launch_tiles_as<64, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace)
                             : launch_tiles_as<128, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace);
   if (a.head_dim == 64) return launch_tiles_as<64, 1, 128, true, false>(ctx, stream, a, min_rows);
-  return keys <= 512 ? launch_tiles_as<128, 1, 128, true, false>(ctx, stream, a, min_rows)
-                     : launch_tiles_as<128, 2, 128, true, false>(ctx, stream, a, min_rows);
+  return (long long)a.max_pages * a.page_size <= 512
+             ? launch_tiles_as<128, 1, 128, true, false>(ctx, stream, a, min_rows)
+             : launch_tiles_as<128, 2, 128, true, false>(ctx, stream, a, min_rows);
 }
 
 }  // namespace adr

@@ -393,6 +393,8 @@ PAGED = [  # new, lens, H, Hk, hd, page, pool layout
     ([3, 8], [3, 2000], 64, 16, 64, 16, "tokens"),                            # 32 rows of a key head
     ([33], [30000], 1, 1, 128, 256, "tokens"),                                # keys shared out among CTAs
     ([50, 1, 1, 60], [9000, 9000, 1, 60], 8, 2, 64, 128, "pairs"),
+    ([1, 300, 1, 33, 200] * 3, [500, 300, 90, 700, 201] * 3, 32, 32, 64, 32, "tokens"),   # both kernels, whole tiles
+    ([1, 100, 100], [9000, 300, 100], 32, 32, 128, 64, "tokens"),                         # both, keys shared out
 ]
 
 
