@@ -35,6 +35,13 @@ namespace {
 
 constexpr int TL_M = 128;   // rows of a tile
 constexpr size_t TL_PARTS_AT = 16384;  // of the workspace: jobs, then parts
+// From this size on, in powers of two, the maximum is subtracted from the scores before the scale is applied.  Below, one
+// fused operation does both, and what the product of maximum and scale loses in fp32 (2^-5 at most) is a factor that a
+// row's probabilities and their sum share; above, it would grow past what fp16 and exp2 hold.
+constexpr float TL_FAR = 0x1p20f;
+__device__ __forceinline__ bool is_far(float base) {  // (not infinity, nor what is not a number)
+  return __float_as_uint(fabsf(base)) - __float_as_uint(TL_FAR) < 0x7F800000u - __float_as_uint(TL_FAR);
+}
 // Of every eight pairs of probabilities, those that the FMA units compute; the others go to the exponential unit.
 constexpr int BY_FMA = 1;
 
@@ -641,9 +648,11 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
           }
           tmem_wait_st();
         }
-        // (a first maximum moves from -infinity: nothing is summed or in O yet but zeros)
-        const bool move = mx > m + slack || (m == -INFINITY && mx > m);
-        if (__any_sync(0xffffffffu, move)) {
+        // (a first maximum moves from -infinity: nothing is summed or in O yet but zeros.  The difference is exact where
+        // it matters; a sum with the slack would round it away in large maxima.)
+        const bool move = mx - m > slack;
+        float base = m * scale2;
+        if (__any_sync(0xffffffffu, move || is_far(base))) {
           const float alpha = move ? (m == -INFINITY ? 0.0f : exp2_fast((m - mx) * scale2)) : 1.0f;
           if (move) m = mx;
           l *= alpha;
@@ -658,8 +667,23 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
               tmem_st_x8(o_at + c, o);
             }
           }
+          base = m * scale2;
+          if (__any_sync(0xffffffffu, is_far(base))) {
+            const float zero = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+            for (int c = 0; c < chunks * 32 && key0 + c < warp_most; c += 8) {
+              uint32_t s[8];
+              tmem_ld_x8(s_at + c, s);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - zero);
+              tmem_st_x8(s_at + c, s);
+            }
+            tmem_wait_st();
+            base = 0.0f;
+          }
         }
-        const float base = m == -INFINITY ? 0.0f : m * scale2;
+        if (m == -INFINITY) base = 0.0f;
         const uint64_t mul = pair_of(scale2, scale2), sub = pair_of(-base, -base);
         uint64_t sum[2] = {0, 0};
         auto powers = [&](const uint32_t (&s)[32], uint32_t (&pk)[16]) {

@@ -1,0 +1,66 @@
+"""Scores where the attention over sequences of different lengths can lose a row: weights far below the largest one, scores
+of many millions, scores that are not finite.  Every form of every kernel, against 64-bit forms."""
+import math
+
+import pytest
+import torch
+
+from adrastea_b200 import MatmulMask
+from serving_oracle import assert_close
+from test_gpu_serving import Pages, gen, half, ints, view
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+# how it is called, new rows, positions, query heads, key heads, head_dim
+FORMS = [("paged", 1, 900, 8, 2, 64), ("paged", 1, 900, 8, 2, 128), ("paged", 1, 9000, 8, 1, 128),  # one row tile, many parts
+         ("paged", 7, 900, 4, 1, 64), ("paged", 7, 900, 4, 1, 128),                                 # 28 rows
+         ("paged", 300, 900, 64, 64, 64), ("paged", 90, 400, 32, 32, 128), ("paged", 300, 900, 64, 64, 128),  # tiles
+         ("paged", 90, 900, 32, 32, 64), ("paged", 300, 900, 32, 32, 128),                          # keys shared out
+         ("paged", 90, 5000, 4, 1, 64), ("paged", 90, 5000, 4, 1, 128),
+         ("packed", 300, 300, 8, 1, 64), ("packed", 300, 300, 8, 1, 128),
+         ("packed", 300, 300, 256, 256, 64), ("packed", 2100, 2100, 3, 1, 128)]                     # small blocks, pairs of tiles
+
+
+def run(kernels, form, q, k, v, scale):
+    """One sequence: q [new, H, hd], k and v [n, Hk, hd], causal."""
+    kind, new, n, H, Hk, hd = form
+    out = torch.full_like(q, 3.0)
+    if kind == "packed":
+        kernels.attention_packed(view(out), view(q), view(k), view(v), ints([0, n]), n, scale, MatmulMask.Causal)
+    else:
+        P = Pages(gen(n), [n], 32, Hk, hd)
+        P.put(0, 0, k, v)
+        kernels.attention_paged(view(out), view(q), P.k, P.v, P.table, ints([0, new]), ints([n]), new, scale,
+                                kernels.attention_paged_workspace(H, Hk, hd))
+    kernels.device_status()
+    return out
+
+
+def first_column(n, H, hd, values):
+    """[n, H, hd], zero but for the first column."""
+    x = torch.zeros((n, H, hd), dtype=torch.float16, device="cuda")
+    x[:, :, 0] = values.half()[:, None] if torch.is_tensor(values) else values
+    return x
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.088])
+def test_scores_of_any_size(kernels, form, scale):
+    """Scores of up to 10^11: whichever key is ahead takes the whole row, and nothing overflows.  (A product of 30000 and a
+    multiple of 16 is exact in fp32; a sum of hd equal ones is off by hd * 2^-24 of it at most, 2 * 10^5 of 5.5 * 10^10 for
+    head_dim 64 and four times as much for 128; two keys that differ do so by 16 * 30000 * hd, 3 and 6 * 10^7.)"""
+    kind, new, n, H, Hk, hd = form
+    g = gen(n + hd)
+    step = torch.randperm(n, device="cuda", generator=g) % 3600 - 1800
+    q = torch.full((new, H, hd), 30000.0, dtype=torch.float16, device="cuda")
+    k = (step * 16).half()[:, None, None].expand(n, Hk, hd).contiguous()
+    v = half(g, n, Hk, hd)
+    out = run(kernels, form, q, k, v, scale)
+    score = step.double() * (1 if scale > 0 else -1)
+    for i in range(0, new, 1 + new // 40):
+        seen = n - new + i + 1
+        ahead = (score[:seen] == score[:seen].max()).nonzero().flatten()   # (equal keys share the row)
+        want = v[ahead].double().mean(0).repeat_interleave(H // Hk, 0)
+        size = v[ahead].double().abs().mean(0).repeat_interleave(H // Hk, 0)
+        assert_close(out[i], want, size * 2.0 ** -11 * 1.05 + want.abs() * 2.0 ** -11 + 2.0 ** -25, i)
