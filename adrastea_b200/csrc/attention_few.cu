@@ -30,6 +30,10 @@ namespace {
 constexpr int FEW_THREADS = 160;       // four computing warps and the producer
 constexpr int MOST_UNITS = 2000000000;  // units of work that can be counted
 
+// Probabilities and their sums are carried times 2^15: fp16 holds that (up to just below 2^16), and what is small keeps as
+// many bits as there are, 11 down to 2^-29 of a row's largest weight and 2^-40 of it below.
+constexpr float FEW_UP = 15.0f;
+
 constexpr int few_kb(int head_dim) { return 8192 / head_dim; }  // 64 keys of 128 columns, 128 of 64
 
 template <int HD, int WM>
@@ -532,10 +536,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         for (int t = 0; t < 2 * G; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[t][i] = exp2_fast(s[t][i] - use_m[i >> 1]);
+            s[t][i] = exp2_fast(s[t][i] - use_m[i >> 1] + FEW_UP);  // (in this order: maxima can be large)
             l[i >> 1] += s[t][i];
           }
-        // probabilities are rounded to fp16 for the tensor cores (2^-11 of each: as much as the output's own rounding)
+        // probabilities are rounded to fp16 for the tensor cores (2^-11 of each, as much as the output's own rounding; see
+        // FEW_UP for the smallest)
         uint32_t pa[G][4];
 #pragma unroll
         for (int g = 0; g < G; ++g) {

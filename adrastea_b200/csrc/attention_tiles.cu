@@ -7,11 +7,12 @@
 //   * producer: Q once, then K and V in blocks of N = 128 (64) keys through a ring of shared-memory slots, by TMA (whole
 //     boxes of rows, or page by page), in the 128-byte swizzle; with N = 64 the tensor-core warp does that too (160
 //     threads: four CTAs to an SM have 96 registers a thread, of 192 they would have 80);
-//   * S = Q K^T by tcgen05.mma into tensor memory; P = exp2(scale2 (S - m)) written back over S by one thread per row;
+//   * S = Q K^T by tcgen05.mma into tensor memory; P = 2^7 exp2(scale2 (S - m)) written back over S by one thread per row;
 //     O += P V with P from tensor memory and V as it lies in memory (N-major), O staying in tensor memory;
 //   * the product with V begins when half a block's probabilities are there;
-//   * the maximum m that a row is scaled by is moved only when a score passes it by more than 2^8 (P then stays within
-//     fp16's range, and the sums are fp32): the rescaling of O in tensor memory is rare;
+//   * the maximum m that a row is scaled by is moved only when a score passes it by more than 2^8: the rescaling of O in
+//     tensor memory is rare.  P and the sums are carried times 2^7, so that they end at 2^15, within fp16's range, and what
+//     is small keeps as many bits as there are: 11 down to 2^-21 of a row's largest weight, 2^-32 of it below;
 //   * when S of a block is complete, so is the product with V before it (the tensor cores run in order), so the softmax
 //     warps may touch O and no further barrier is needed;
 //   * few tiles over many pages: the keys of each are shared out among CTAs, and a second kernel joins the parts.
@@ -35,6 +36,8 @@ namespace {
 
 constexpr int TL_M = 128;   // rows of a tile
 constexpr size_t TL_PARTS_AT = 16384;  // of the workspace: jobs, then parts
+// Probabilities are at most 2^8 (see above); fp16 holds up to just below 2^16.
+constexpr float TL_UP = 7.0f;
 // From this size on, in powers of two, the maximum is subtracted from the scores before the scale is applied.  Below, one
 // fused operation does both, and what the product of maximum and scale loses in fp32 (2^-5 at most) is a factor that a
 // row's probabilities and their sum share; above, it would grow past what fp16 and exp2 hold.
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
           }
         }
         if (m == -INFINITY) base = 0.0f;
-        const uint64_t mul = pair_of(scale2, scale2), sub = pair_of(-base, -base);
+        const uint64_t mul = pair_of(scale2, scale2), sub = pair_of(TL_UP - base, TL_UP - base);
         uint64_t sum[2] = {0, 0};
         auto powers = [&](const uint32_t (&s)[32], uint32_t (&pk)[16]) {
 #pragma unroll

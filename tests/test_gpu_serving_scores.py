@@ -45,6 +45,31 @@ def first_column(n, H, hd, values):
 
 
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("x", [9.5, 14.875, 17.0, 18.0])
+def test_many_small_weights_count(kernels, form, x):
+    """One key takes the most and all others e^-x of it each, as after a first token that every row looks at: together they
+    are the output, because the first value is zero.
+
+    Bound: a weight is rounded to fp16, 2^-11 of it, or 2^-32 of the row's largest where that is more; the exponential is
+    good to 2^-18 and to 2^-21 of x; the sums' roundings, of 2^-24 each, are the factor 1.05; the output is rounded to
+    fp16."""
+    kind, new, n, H, Hk, hd = form
+    big = 1024.0
+    k = first_column(n, Hk, hd, torch.full((n,), -x, device="cuda"))
+    k[0] = 0
+    v = torch.full((n, Hk, hd), big, dtype=torch.float16, device="cuda")
+    v[0] = 0
+    out = run(kernels, form, first_column(new, H, hd, 1.0), k, v, 1.0)
+    others = torch.arange(n - new, n, dtype=torch.float64, device="cuda")[:, None, None].expand(new, H, hd)
+    p = math.exp(-x)
+    l = 1 + others * p
+    want = others * p * big / l
+    tol = 1.05 * others * big / l * (max(p * 2.0 ** -11, 2.0 ** -32) + p * (2.0 ** -18 + 2.0 ** -21 * x)) \
+        + want * 2.0 ** -11 + 2.0 ** -25
+    assert_close(out, want, tol)
+
+
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("scale", [1.0, -1.0, 0.088])
 def test_scores_of_any_size(kernels, form, scale):
     """Scores of up to 10^11: whichever key is ahead takes the whole row, and nothing overflows.  (A product of 30000 and a
@@ -64,3 +89,10 @@ def test_scores_of_any_size(kernels, form, scale):
         want = v[ahead].double().mean(0).repeat_interleave(H // Hk, 0)
         size = v[ahead].double().abs().mean(0).repeat_interleave(H // Hk, 0)
         assert_close(out[i], want, size * 2.0 ** -11 * 1.05 + want.abs() * 2.0 ** -11 + 2.0 ** -25, i)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("scale", [2.5e-3, 1.25e-3, 3e-4, -1e-5])
+def test_scores_where_fp32_takes_steps_like_the_weights(kernels, form, scale):
+    """Scores of 10^8 down to 10^6 with steps of 16 to 1/8 between them in fp32."""
+    test_scores_of_any_size(kernels, form, scale)
