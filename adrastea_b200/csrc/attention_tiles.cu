@@ -800,8 +800,9 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
     }
     if (SPLIT && ok && live) p.part_ml[(size_t)blockIdx.x * TL_M + row] = make_float2(m * scale2, l);
     if (ok && warp_live) {
-      // a row that sees no key gets zeros
-      const float inv = limit > 0 ? 1.0f / l : 0.0f;
+      // A row that sees no key gets zeros; one whose scores are all -infinity has no softmax, and is not a number.  (Its sum
+      // is not zero: see exp2_fma2.)
+      const float inv = limit > 0 ? 1.0f / (m == -INFINITY ? 0.0f : l) : 0.0f;
       __half* dst = p.a.out + (long long)(span.q0 + first + tok) * p.a.so[0] +
                     (long long)(head * p.a.group + row - tok * p.a.group) * p.a.so[1];
 #pragma unroll

@@ -96,3 +96,24 @@ def test_scores_of_any_size(kernels, form, scale):
 def test_scores_where_fp32_takes_steps_like_the_weights(kernels, form, scale):
     """Scores of 10^8 down to 10^6 with steps of 16 to 1/8 between them in fp32."""
     test_scores_of_any_size(kernels, form, scale)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("finite", [False, True])
+def test_scores_of_minus_infinity(kernels, form, finite):
+    """Keys with a score of -infinity have no weight; a row that sees no others has no softmax: not a number, in whichever
+    kernel it is.  (Rows from the middle one on see keys of a finite score where there are such.)"""
+    kind, new, n, H, Hk, hd = form
+    k = first_column(n, Hk, hd, -INF)
+    v = half(gen(n), n, Hk, hd)
+    none = new // 2 if finite else new   # rows that see no finite score
+    first = n - new + none
+    k[first:] = 0
+    out = run(kernels, form, first_column(new, H, hd, 1.0), k, v, 1.0)
+    assert out[:none].isnan().all()
+    rows = torch.arange(1, new - none + 1, device="cuda", dtype=torch.float64)[:, None, None]
+    vs = v[first:].double()
+    want = (vs.cumsum(0) / rows).repeat_interleave(H // Hk, 1)
+    size = (vs.abs().cumsum(0) / rows).repeat_interleave(H // Hk, 1)
+    # equal weights of 1, which fp16 holds; fp32 sums of up to 2100 of them
+    assert_close(out[none:], want, size * 2100 * 2.0 ** -24 + size * 2.0 ** -11 + want.abs() * 2.0 ** -11 + 2.0 ** -25)
