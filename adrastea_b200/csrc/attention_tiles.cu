@@ -565,10 +565,10 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
     const int my_end = NT == 2 && t == 1 ? kend[NT - 1] : kend[0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + (uint32_t)(t * N), o_at = tmem + lanes + Cfg::O_COL + (uint32_t)(t * HD);
-    // scores in powers of two; the sign of the scale goes into the scores so that the largest product is the maximum
-    // (a scale of zero, which would make NaN of what is masked, is as good as one of 1e-30: exp2 is 1 for every score)
+    // scores in powers of two; the sign of the scale, and a scale of zero, go into the scores, so that the largest product is
+    // the maximum, what is masked stays infinite, and zero times infinity is not a number
     const float scale2 = fmaxf(fabsf(p.a.scale) * 1.4426950408889634f, 1e-30f);
-    const bool negative = p.a.scale < 0.0f;
+    const float sign = p.a.scale > 0.0f ? 1.0f : p.a.scale < 0.0f ? -1.0f : 0.0f;
     const float slack = 8.0f / scale2;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
         const int chunks = partly ? (min(N, my_end - key0) + 31) / 32 : N / 32;  // of 32 keys
         // the row's maximum
         float mx;
-        if (!partly && !negative) {
+        if (!partly && sign == 1.0f) {
           uint32_t s[N];
 #pragma unroll
           for (int c = 0; c < N / 32; ++c) tmem_ld_x32(s_at + c * 32, s + c * 32);
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              if (negative) s[i] ^= 0x80000000u;
+              s[i] = __float_as_uint(__uint_as_float(s[i]) * sign);
               if (k + i >= limit) s[i] = 0xFF800000u;  // -infinity
               mx = fmaxf(mx, __uint_as_float(s[i]));
             }

@@ -117,3 +117,16 @@ def test_scores_of_minus_infinity(kernels, form, finite):
     size = (vs.abs().cumsum(0) / rows).repeat_interleave(H // Hk, 1)
     # equal weights of 1, which fp16 holds; fp32 sums of up to 2100 of them
     assert_close(out[none:], want, size * 2100 * 2.0 ** -24 + size * 2.0 ** -11 + want.abs() * 2.0 ** -11 + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("value", [INF, -INF])
+def test_infinite_scores_times_a_scale_of_zero(kernels, form, value):
+    """0 * infinity is not a number: so are the rows that see that key, and no others."""
+    kind, new, n, H, Hk, hd = form
+    k = first_column(n, Hk, hd, 1.0)
+    at = n - new + new // 2
+    k[at, :, 0] = value
+    v = half(gen(n), n, Hk, hd)
+    out = run(kernels, form, first_column(new, H, hd, 1.0), k, v, 0.0)
+    assert out[new // 2:].isnan().all() and out[:new // 2].isfinite().all()
