@@ -111,17 +111,30 @@ class PagedCache:
             raise MemoryError("a sequence is longer than its row of the block table")
         if sum(need) > len(self.free):
             raise MemoryError(f"{sum(need)} pages wanted, {len(self.free)} free")
-        for s, n, m in zip(seqs, new, need):
-            if m > 0:
-                at, got = len(self.pages[s]), [self.free.pop() for _ in range(m)]
-                self.pages[s] += got
-                self.table[s, at:at + m] = torch.tensor(got, dtype=torch.int32, device=self.device)
+        # (what can fail comes before the books: entries of the table behind a sequence's end are not read)
+        left = len(self.free) - sum(need)
+        pages = reversed(self.free[left:])
+        got = [[next(pages) for _ in range(m)] for m in need]
+        for s, row in zip(seqs, got):
+            if row:
+                at = len(self.pages[s])
+                self.table[s, at:at + len(row)] = torch.tensor(row, dtype=torch.int32, device=self.device)
+        del self.free[left:]
+        for s, n, row in zip(seqs, new, got):
+            self.pages[s] += row
             self.length[s] += n
 
-    def release(self, seq: int):
+    def truncate(self, seq: int, length: int):
+        """Positions from `length` on are given up, and with them the pages behind the last one."""
         assert 0 <= seq < len(self.length), "no such sequence slot"
-        self.free += reversed(self.pages[seq])
-        self.pages[seq], self.length[seq] = [], 0
+        assert 0 <= length <= self.length[seq], f"the sequence has {self.length[seq]} positions"
+        keep = -(-length // self.page_size)
+        self.free += reversed(self.pages[seq][keep:])
+        del self.pages[seq][keep:]
+        self.length[seq] = length
+
+    def release(self, seq: int):
+        self.truncate(seq, 0)
 
 
 class LlamaU8Layer:
@@ -449,19 +462,19 @@ class LlamaU8:
     def extend(self, cache: PagedCache, seqs: list[int], tokens: list[torch.Tensor]) -> torch.Tensor:
         """tokens[i] (int64, at least one) go behind what the cache holds of sequence slot seqs[i]: whole prompts,
         chunks of them and single tokens in any mixture, all rows through each layer at once.  Returns the argmax
-        behind every sequence's last token; self.logits[:len(seqs)] holds the logits."""
+        behind every sequence's last token; self.logits[:len(seqs)] holds the logits.  A step that fails, whatever
+        the reason, leaves the sequences as long as they were."""
         sh, n = self.shape, len(seqs)
         assert 0 < n <= self.B and self.fused_attention and all(t.numel() > 0 for t in tokens)
         new = [t.numel() for t in tokens]
-        cache.extend(seqs, new)
         ints = lambda x: torch.tensor(x, dtype=torch.int32, device=self.device)
         starts = [0]
         for m in new:
             starts.append(starts[-1] + m)
         T, hd, Hl, d, dl, fl = starts[-1], sh.head_dim, self.Hl, sh.dim, self.dl, self.fl
-        cu_q, kv_len, table = ints(starts), ints([cache.length[s] for s in seqs]), cache.table[seqs]
         if self._rope is None:
             self._rope = self.k.rope_table(hd, sh.theta)
+        if self._attention_ws is None:
             self._attention_ws = self.k.attention_paged_workspace(Hl, Hl, hd)
         f16 = dict(dtype=torch.float16, device=self.device)
         h = self.embed[torch.cat([t.reshape(-1) for t in tokens])].clone()
@@ -470,21 +483,29 @@ class LlamaU8:
         gu, g = torch.zeros((T, 2 * fl), **f16), torch.empty((T, fl), **f16)
         heads = lambda t: TensorView.of(t.unflatten(1, (Hl, hd)))
         q, k, v = (heads(t) for t in qkv.split(dl, 1))
-        for li, ly in enumerate(self.layers):
-            self._norm(x, h, ly.attn_norm)
-            self._prefill_linear(ly.wqkv, qkv, x)
-            self.k.rope_append_paged(q, q, k, v, cache.k[li], cache.v[li], table, cu_q, kv_len, self._rope)
-            self.k.attention_paged(heads(att), q, cache.k[li], cache.v[li], table, cu_q, kv_len, max(new),
-                                   1.0 / math.sqrt(hd), self._attention_ws)
-            self._prefill_linear(ly.wo, h, att, part, residual=True)
-            self._norm(x, h, ly.ffn_norm)
-            self._prefill_linear(ly.wgu, gu, x)
-            self._silu_mul(g, gu)
-            self._prefill_linear(ly.down, h, g, part, residual=True)
-        last = h[cu_q[1:].long() - 1]
-        self._norm(self.x[:n], last, self.out_norm)
-        self.k.matmul_nt_fp16u8(self.logits[:n], self.x[:n], self.lm_head.q, self.lm_head.scales, self.lm_head.block)
-        return torch.argmax(self.logits[:n], dim=-1)
+        cu_q, before = ints(starts), list(cache.length)
+        cache.extend(seqs, new)
+        try:
+            kv_len, table = ints([cache.length[s] for s in seqs]), cache.table[seqs]
+            for li, ly in enumerate(self.layers):
+                self._norm(x, h, ly.attn_norm)
+                self._prefill_linear(ly.wqkv, qkv, x)
+                self.k.rope_append_paged(q, q, k, v, cache.k[li], cache.v[li], table, cu_q, kv_len, self._rope)
+                self.k.attention_paged(heads(att), q, cache.k[li], cache.v[li], table, cu_q, kv_len, max(new),
+                                       1.0 / math.sqrt(hd), self._attention_ws)
+                self._prefill_linear(ly.wo, h, att, part, residual=True)
+                self._norm(x, h, ly.ffn_norm)
+                self._prefill_linear(ly.wgu, gu, x)
+                self._silu_mul(g, gu)
+                self._prefill_linear(ly.down, h, g, part, residual=True)
+            last = h[cu_q[1:].long() - 1]
+            self._norm(self.x[:n], last, self.out_norm)
+            self.k.matmul_nt_fp16u8(self.logits[:n], self.x[:n], self.lm_head.q, self.lm_head.scales, self.lm_head.block)
+            return torch.argmax(self.logits[:n], dim=-1)
+        except BaseException:
+            for s in reversed(seqs):  # (pages go back in the order that they would be taken in again)
+                cache.truncate(s, before[s])
+            raise
 
 
 def main():

@@ -1,0 +1,100 @@
+"""What fails on the way leaves the paged cache and the harness as they were, and sizes that C's int does not hold are
+refused.  No GPU: the kernels are a stand-in, on tensors of the host."""
+from unittest import mock
+
+import pytest
+import torch
+
+from adrastea_b200 import AdrError, RopeLayout, RopeTable, kernels as K
+from adrastea_b200.llama import LlamaShape, LlamaU8, PagedCache
+
+
+def state(c):
+    return [list(p) for p in c.pages], list(c.length), list(c.free)
+
+
+def model():
+    shape = LlamaShape(dim=128, n_heads=2, ffn=64, n_layers=2, vocab=64, block=64)
+    return LlamaU8(mock.MagicMock(), shape, max_batch=3, max_seq=64, device="cpu")
+
+
+def test_a_table_that_cannot_be_written_leaves_the_cache_alone(monkeypatch):
+    c = PagedCache(1, 8, 16, 1, 8, 3, 64, device="cpu")
+    c.extend([0], [20])
+    before, real, calls = state(c), torch.tensor, []
+
+    def second_fails(*a, **kw):
+        calls.append(0)
+        if len(calls) == 2:
+            raise torch.OutOfMemoryError("no memory")
+        return real(*a, **kw)
+
+    monkeypatch.setattr(torch, "tensor", second_fails)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.extend([0, 1, 2], [20, 20, 20])
+    monkeypatch.setattr(torch, "tensor", real)
+    assert state(c) == before
+    c.extend([0, 1, 2], [20, 20, 20])
+    assert c.length == [40, 20, 20] and sorted(sum(c.pages, []) + c.free) == list(range(8))
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "matmul_nt_fp16u8", "rope_append_paged", "attention_paged",
+                                  "attention_paged_workspace", "elementwise_binary_2d_f16"])
+def test_a_step_that_fails_gives_its_positions_back(name):
+    m = model()
+    c = m.paged_cache(pages=9, page_size=16)
+    toks = [torch.arange(20), torch.arange(3)]
+    m.extend(c, [0, 2], toks)
+    before = state(c)
+    getattr(m.k, name).side_effect = AdrError(4, "refused")
+    m._attention_ws = None
+    with pytest.raises(AdrError):
+        m.extend(c, [2, 0], [torch.arange(30), torch.arange(17)])
+    assert state(c) == before
+    getattr(m.k, name).side_effect = None
+    m.extend(c, [2, 0], [torch.arange(30), torch.arange(17)])
+    assert c.length == [37, 0, 33]
+
+
+@pytest.mark.parametrize("tokens", [[torch.arange(20), torch.zeros(0, dtype=torch.int64)],   # none for the second
+                                    [torch.arange(20), torch.tensor([64])],                  # no such row of the embedding
+                                    [torch.arange(20)],                                      # one list too short
+                                    [torch.arange(20), torch.arange(60)]])                   # more pages than there are
+def test_tokens_that_are_refused_take_no_pages(tokens):
+    m = model()
+    c = m.paged_cache(pages=5, page_size=16)
+    before = state(c)
+    with pytest.raises((AssertionError, IndexError, MemoryError)):
+        m.extend(c, [0, 1], tokens)
+    assert state(c) == before
+
+
+def test_truncated_sequences_give_back_the_pages_behind_their_end():
+    c = PagedCache(1, 8, 4, 1, 8, 2, 32, device="cpu")
+    c.extend([0, 1], [10, 3])
+    c.truncate(0, 5)
+    assert c.length == [5, 3] and len(c.pages[0]) == 2 and len(c.free) == 5
+    c.truncate(0, 4)
+    assert c.length[0] == 4 and len(c.pages[0]) == 1
+    c.extend([0], [5])
+    assert c.table[0, :3].tolist() == c.pages[0] and not set(c.pages[0]) & set(c.pages[1] + c.free)
+    c.truncate(0, 0)
+    assert c.pages[0] == [] and len(c.free) == 7
+    for bad in (-1, 4):
+        with pytest.raises(AssertionError):
+            c.truncate(1, bad)
+    with pytest.raises(AssertionError):
+        c.truncate(2, 0)
+
+
+# ------------------------------------------------------------------ sizes
+MANY = 1 << 32   # C's int would make 0 of it, and of MANY + 5 five
+
+
+def rows(*dims):
+    """Dimensions and the strides of a contiguous view."""
+    s, strides = 1, []
+    for d in reversed(dims):
+        strides.append(s)
+        s *= d
+    return dims, tuple(reversed(strides))
