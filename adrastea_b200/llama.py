@@ -209,6 +209,7 @@ class LlamaU8:
         self._graph = None
         self._deq = None  # fp16 scratch for one expanded weight matrix (prefill)
         self._rope = self._attention_ws = None  # table and workspace of `extend`
+        self._foreign_logits = False  # the rows of self.logits are those of other sequences
         # rms_norm inside the decode product that follows it (adr_rms_norm_matmul_nt_fp16u8,
         # adr_rms_norm_silu_mul_matmul_nt_fp16u8: same bits, one launch fewer per norm), for the
         # batches of up to four that run on that kernel: 16 layers of the 7B shape at 575 positions
@@ -341,8 +342,16 @@ class LlamaU8:
         with torch.cuda.graph(self._graph):
             self._decode_step_body()
 
+    def _clear_logits(self):
+        """The u8 products read what they overwrite (beta * old, even for beta = 0), so logits that are not numbers would
+        be those of whichever sequence has the row next."""
+        if self._foreign_logits:
+            self.logits.zero_()
+            self._foreign_logits = False
+
     def decode_step(self):
         """Consumes self.tokens at position self.pos, leaves the argmax in self.next_tokens."""
+        self._clear_logits()
         if self._graph is not None:
             self._graph.replay()
         else:
@@ -446,6 +455,8 @@ class LlamaU8:
             self._prefill_linear(ly.down, h, g, part, residual=True)
         last = h.view(B, S0, d)[:, -1].contiguous()
         self._norm(self.x, last, self.out_norm)
+        self._foreign_logits = True
+        self._clear_logits()
         self.k.matmul_nt_fp16u8(self.logits, self.x, self.lm_head.q, self.lm_head.scales, self.lm_head.block)
         self.tokens.copy_(torch.argmax(self.logits, dim=-1))
         self.pos.fill_(S0)
@@ -500,7 +511,10 @@ class LlamaU8:
                 self._prefill_linear(ly.down, h, g, part, residual=True)
             last = h[cu_q[1:].long() - 1]
             self._norm(self.x[:n], last, self.out_norm)
+            self._foreign_logits = True
+            self._clear_logits()
             self.k.matmul_nt_fp16u8(self.logits[:n], self.x[:n], self.lm_head.q, self.lm_head.scales, self.lm_head.block)
+            self._foreign_logits = True  # (for a decode step of the rectangular cache)
             return torch.argmax(self.logits[:n], dim=-1)
         except BaseException:
             for s in reversed(seqs):  # (pages go back in the order that they would be taken in again)

@@ -11,6 +11,43 @@ from test_gpu_serving import Pages, chain, gen, half, ints, paged_case, starts, 
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_logits_of_a_step_do_not_see_those_of_the_step_before(kernels, captured):
+    """A request whose logits are not numbers does not spoil the next one in its row of the output: not of `extend`, not of
+    a new prompt, not of a token of the rectangular cache."""
+    shape = LlamaShape(dim=256, n_heads=2, ffn=512, n_layers=1, vocab=512, block=64)
+    toks = torch.randint(0, shape.vocab, (2, 9), device="cuda", generator=gen(1))
+    bad = torch.full((2, 1), 3, dtype=torch.int64, device="cuda")
+
+    def run(spoil):
+        model = LlamaU8(kernels, shape, max_batch=2, max_seq=64, seed=5)
+        toks[toks == 3] = 4
+        model.embed[3] = float("nan") if spoil else 0.0
+        cache, got = model.paged_cache(pages=16, page_size=16, max_seqs=4), []
+
+        def spoiled():
+            model.extend(cache, [2, 3], list(bad))
+            assert model.logits.isnan().all() == spoil
+
+        if captured:
+            model.prefill(toks)
+            model.capture()
+        spoiled()
+        model.extend(cache, [0, 1], list(toks))
+        got.append(model.logits.clone())
+        spoiled()
+        model.prefill(toks)
+        got.append(model.logits.clone())
+        model.tokens.clamp_(min=4)
+        spoiled()
+        model.decode_step()
+        got.append(model.logits.clone())
+        return got
+
+    for want, got in zip(run(False), run(True)):
+        assert want.isfinite().all() and torch.equal(want, got)
+
+
 def test_a_step_that_fails_is_as_if_it_had_not_been(kernels, monkeypatch):
     """A launch in the middle of a step is refused: the sequences are as long as before, and the step, taken again, gives
     what it gives in a run without the failure."""
