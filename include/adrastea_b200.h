@@ -509,9 +509,10 @@ int adr_attention_f16(adr_ctx* ctx, adr_stream stream, void* out, const void* q,
  * slot * strides[1] + head * strides[2] + column (elements, 64-bit, not negative).  Query head h
  * belongs to key head h / (n_heads / n_kv_heads).  What the arrays hold is checked on the device:
  * rows are cut to `tokens`, lengths to max_pages * page_size, and a page outside the pool is not
- * written and reads as zeros; each of the last two, a row at a negative position, and sequences whose
- * rows overlap so much that the attention over pages leaves them undone, also set the word behind
- * adr_device_status.  A tensor may not overlap one that the same call writes, unless
+ * written and reads as zeros; each of the last two, and a row appended at a negative position, also set
+ * the word behind adr_device_status.  Of sequences whose rows overlap (cu_q falls somewhere) the attention
+ * may leave some undone; the word says so where max_q stands for up to 32 rows of a key head, and
+ * need not elsewhere.  A tensor may not overlap one that the same call writes, unless
  * its entry says so; two sequences may share pages that neither writes.
  * ------------------------------------------------------------------------ */
 

@@ -11,6 +11,46 @@ from test_gpu_serving import Pages, chain, gen, half, ints, paged_case, starts, 
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("n,T,H,Hk,hd", [(64, 2048, 32, 8, 64), (31, 2048, 8, 8, 128), (200, 300, 4, 4, 64), (9, 130, 2, 1, 128)])
+def test_tiles_of_overlapping_sequences(kernels, paged, n, T, H, Hk, hd):
+    """Every second sequence claims all rows: more tiles than sequences side by side can have.  What is written are rows of
+    those sequences, nothing beside them; the next call is as ever."""
+    g, page = gen(n), 16
+    q, k, v = half(g, T, H, hd), half(g, T, Hk, hd), half(g, T, Hk, hd)
+    P = Pages(g, [1024], page, Hk, hd)
+    keys, values = half(g, 1024, Hk, hd), half(g, 1024, Hk, hd)
+    P.put(0, 0, keys, values)
+    table = P.table[:, :-1].expand(n, -1).contiguous()
+    store, ws = torch.full((T + 20, H, hd), 2.0, dtype=torch.float16, device="cuda"), kernels.attention_paged_workspace(H, Hk, hd)
+    out = store[10:-10]
+
+    def call(cu, lens, max_q):
+        if paged:
+            kernels.attention_paged(view(out), view(q), P.k, P.v, table, ints(cu), ints(lens), max_q, 0.1, ws)
+        else:
+            kernels.attention_packed(view(out), view(q), view(k), view(v), ints(cu), max_q, 0.1)
+
+    def check(rows, may_be_undone):
+        m = rows.stop - rows.start
+        want, tol = attend(q[rows], *((keys, values, 0.1, 1024 - m + 1) if paged else (k[rows], v[rows], 0.1, 1)))
+        done = (out[rows] != 2.0).any(-1, keepdim=True) if may_be_undone else torch.ones_like(want[..., :1], dtype=torch.bool)
+        assert_close(torch.where(done, out[rows].double(), 0.0), torch.where(done, want, 0.0), tol)
+
+    call([T * (s % 2) for s in range(n + 1)], [1024] * n, T)
+    try:
+        kernels.device_status()   # (it may say so, and need not)
+    except AdrError:
+        pass
+    check(slice(0, T), True)
+    cu = [T * s // n for s in range(n + 1)]
+    call(cu, [1024] * n, max(b - a for a, b in zip(cu, cu[1:])))
+    kernels.device_status()
+    for a, b in zip(cu, cu[1:]):
+        check(slice(a, b), False)
+    assert (store[:10] == 2.0).all() and (store[-10:] == 2.0).all()
+
+
 @pytest.mark.parametrize("captured", [False, True])
 def test_logits_of_a_step_do_not_see_those_of_the_step_before(kernels, captured):
     """A request whose logits are not numbers does not spoil the next one in its row of the output: not of `extend`, not of
