@@ -360,7 +360,7 @@ extern "C" int adr_rope_f16(adr_ctx* ctx, adr_stream stream, void* out, const vo
   const RopePlan r{reinterpret_cast<const unsigned long long*>(turns), rotary_dim, amplitude, head_dim};
   const Strided so{strides_o[0], strides_o[1]}, si{strides_i[0], strides_i[1]};
   auto go = [&](auto kfn, int per) {
-    return launch_rows(ctx, (cudaStream_t)stream, kfn, (tokens + per - 1) / per, (__half*)out, (const __half*)in, so, si,
+    return launch_rows(ctx, (cudaStream_t)stream, kfn, (tokens - 1) / per + 1, (__half*)out, (const __half*)in, so, si,
                        tokens, n_heads, (const int*)positions, r);
   };
   const bool many = vec && many_rows(ctx, tokens), half = layout == ADR_ROPE_HALF;
@@ -414,7 +414,7 @@ extern "C" int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_ou
   p.n_pages = n_pages;
   p.r = {reinterpret_cast<const unsigned long long*>(turns), rotary_dim, amplitude, head_dim};
   p.status = ctx->d_status;
-  auto go = [&](auto kfn, int per) { return launch_rows(ctx, (cudaStream_t)stream, kfn, (tokens + per - 1) / per, p); };
+  auto go = [&](auto kfn, int per) { return launch_rows(ctx, (cudaStream_t)stream, kfn, (tokens - 1) / per + 1, p); };
   const bool many = vec && many_rows(ctx, tokens), half = layout == ADR_ROPE_HALF;
   if (many)
     return half ? go(rope_append_kernel<true, true, ROPE_MANY>, ROPE_MANY)

@@ -51,6 +51,24 @@ def test_tiles_of_overlapping_sequences(kernels, paged, n, T, H, Hk, hd):
     assert (store[:10] == 2.0).all() and (store[-10:] == 2.0).all()
 
 
+def test_as_many_rows_as_there_are_positions(kernels):
+    """2^31 - 1 rows in one call (34 GB, in place)."""
+    T = (1 << 31) - 1
+    g = gen(8)
+    x = torch.zeros((T, 1, 8), dtype=torch.float16, device="cuda")
+    ends = [slice(0, 5), slice(T - 5, T)]
+    before = [half(g, 5, 1, 8) for _ in ends]
+    for at, b in zip(ends, before):
+        x[at] = b
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    table = kernels.rope_table(8, 10000.0, RopeLayout.Interleaved)
+    kernels.rope_f16(view(x), view(x), pos, table)
+    for at, b in zip(ends, before):
+        assert_close(x[at], *rotate(b, pos[at], 8, 10000.0, False, RopeScaling()))
+    del x, pos
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("captured", [False, True])
 def test_logits_of_a_step_do_not_see_those_of_the_step_before(kernels, captured):
     """A request whose logits are not numbers does not spoil the next one in its row of the output: not of `extend`, not of
