@@ -266,9 +266,15 @@ _f16 = torch.float16
 
 # The serving operators are called once per layer and step, for kernels of a few microseconds.  What follows from the
 # dimensions and strides of a call's arguments is worked out once for all calls with the same ones.
+def _sizes(what: str, dims: tuple):
+    """The library takes sizes as C ints, of which ctypes keeps the low 32 bits without a word."""
+    assert max(dims) < 1 << 31, f"{what} is {tuple(dims)}: a call takes at most 2^31 - 1 of each"
+
+
 def _rows(what: str, dims: tuple, strides: tuple, want: tuple):
     """The token and head strides of a [tokens, heads, head_dim] view."""
     assert dims == want, f"{what} must be {tuple(want)}, is {tuple(dims)}"
+    _sizes(what, dims)
     assert strides[2] == 1 or dims[2] == 1, f"the columns of {what} must follow one another"
     return (C.c_longlong * 2)(*strides[:2])
 
@@ -276,6 +282,7 @@ def _rows(what: str, dims: tuple, strides: tuple, want: tuple):
 def _pool(what: str, dims: tuple, strides: tuple, want: tuple):
     """The page, slot and head strides of a [pages, page_size, kv_heads, head_dim] tensor."""
     assert dims == want and strides[3] == 1, f"{what} must be {tuple(want)} with unit column stride"
+    _sizes(what, dims)
     return (C.c_longlong * 3)(*strides[:3])
 
 
@@ -291,6 +298,7 @@ def _packed_plan(out, s_out, q, s_q, k, s_k, v, s_v, cu_q):
     T, H, hd = q
     Hk = k[-2]
     assert len(cu_q) == 1, "cu_q must be [sequences + 1]"
+    _sizes("cu_q", cu_q)
     return (T, cu_q[0] - 1, H, Hk, hd, _rows("output", out, s_out, q), _rows("q", q, s_q, q),
             _rows("k", k, s_k, (T, Hk, hd)), _rows("v", v, s_v, (T, Hk, hd)))
 
@@ -298,6 +306,7 @@ def _packed_plan(out, s_out, q, s_q, k, s_k, v, s_v, cu_q):
 def _tables(table: tuple, cu_q: tuple, kv_len: tuple):
     assert len(kv_len) == 1 and len(table) == 2 and table[0] == kv_len[0] and cu_q == (kv_len[0] + 1,), \
         f"block_table [n, max_pages], cu_q [n + 1] and kv_len [n] are {tuple(table)}, {tuple(cu_q)}, {tuple(kv_len)}"
+    _sizes("block_table", table)
 
 
 @functools.lru_cache(maxsize=4096)

@@ -98,3 +98,31 @@ def rows(*dims):
         strides.append(s)
         s *= d
     return dims, tuple(reversed(strides))
+
+
+@pytest.mark.parametrize("T,H", [(MANY + 5, 1), (1 << 31, 1), (2, MANY + 1)])
+def test_rows_that_an_int_does_not_hold_are_refused(T, H):
+    x, s = rows(T, H, 8)
+    with pytest.raises(AssertionError):
+        K._rope_plan(x, s, x, s, (T,))
+    x, s = rows(T, H, 64)
+    with pytest.raises(AssertionError):
+        K._packed_plan(x, s, x, s, x, s, x, s, (3,))
+
+
+@pytest.mark.parametrize("pages,sequences,columns", [(MANY + 5, 2, 4), (9, MANY + 2, 4), (9, 2, MANY + 4)])
+def test_pages_and_tables_that_an_int_does_not_hold_are_refused(pages, sequences, columns):
+    x, s = rows(6, 4, 64)
+    kv, skv = rows(6, 2, 64)
+    pool, sp = rows(pages, 16, 2, 64)
+    tables = (sequences, columns), (sequences + 1,), (sequences,)
+    with pytest.raises(AssertionError):
+        K._append_plan(x, s, x, s, kv, skv, kv, skv, pool, sp, pool, sp, *tables)
+    with pytest.raises(AssertionError):
+        K._paged_plan(x, s, x, s, pool, sp, pool, sp, *tables)
+
+
+def test_largest_rows_are_taken():
+    T = (1 << 31) - 1
+    x, s = rows(T, 1, 8)
+    assert K._rope_plan(x, s, x, s, (T,))[:3] == (T, 1, 8)
