@@ -206,6 +206,12 @@ class RopeTable:
     layout: RopeLayout
     amplitude: float
 
+    def __post_init__(self):  # (the kernels read that many, whatever the table's size)
+        assert self.turns.shape == (self.rotary_dim // 2,) and self.rotary_dim % 2 == 0, \
+            f"a table of {self.rotary_dim} columns has half as many turns, not {tuple(self.turns.shape)}"
+        if self.turns.dtype is not torch.int64:
+            raise TypeError(f"the turns must be torch.int64, got {self.turns.dtype}")
+
 
 def lower_matmul(output: TensorView, left: TensorView, right: TensorView,
                  options: MatmulOptions) -> tuple:

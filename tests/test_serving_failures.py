@@ -126,3 +126,16 @@ def test_largest_rows_are_taken():
     T = (1 << 31) - 1
     x, s = rows(T, 1, 8)
     assert K._rope_plan(x, s, x, s, (T,))[:3] == (T, 1, 8)
+
+
+@pytest.mark.parametrize("turns,rotary", [(torch.zeros(31, dtype=torch.int64), 64), (torch.zeros(64, dtype=torch.int64), 64),
+                                          (torch.zeros((32, 1), dtype=torch.int64), 64), (torch.zeros(32), 64),
+                                          (torch.zeros(32, dtype=torch.int64), 65)])
+def test_a_table_of_another_size_is_refused(turns, rotary):
+    """The kernels read rotary_dim / 2 numbers of it."""
+    with pytest.raises((AssertionError, TypeError)):
+        RopeTable(turns, rotary, RopeLayout.Half, 1.0)
+
+
+def test_a_table_of_the_right_size_is_taken():
+    assert RopeTable(torch.zeros(32, dtype=torch.int64), 64, RopeLayout.Half, 1.0).rotary_dim == 64
