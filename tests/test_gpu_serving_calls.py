@@ -11,6 +11,82 @@ from test_gpu_serving import Pages, chain, gen, half, ints, paged_case, starts, 
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("pdl", [0, 1])
+@pytest.mark.parametrize("m", [1, 2, 40])
+def test_a_replayed_step_appends_what_it_is_given(kernels, pdl, m):
+    """Lengths, the pages' order and the projections change between replays: the rotated queries, the slots that are written
+    and all those that are not, and the attention follow what the arrays hold at the replay."""
+    kernels.set_tunable("pdl", pdl)
+    try:
+        H, Hk, hd, page, n, most = 8, 2, 128, 16, 3, 1000
+        g = gen(m)
+        P = Pages(g, [most] * n, page, Hk, hd, fill=0.0)
+        f16 = dict(dtype=torch.float16, device="cuda")
+        st = dict(H=H, Hk=Hk, qkv=half(g, n * m, H + 2 * Hk, hd), q=torch.empty((n * m, H, hd), **f16), P=P,
+                  cu=ints([i * m for i in range(n + 1)]), lens=ints([most] * n), rope=kernels.rope_table(hd, 10000.0), max_q=m,
+                  scale=0.1, ws=kernels.attention_paged_workspace(H, Hk, hd), out=torch.empty((n * m, H, hd), **f16))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            chain(kernels, st)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            chain(kernels, st)
+        for lens in ([100, 40, 1000], [m, 999, 64], [777, 50, 333]):
+            order = torch.randperm(P.n, device="cuda", generator=g).to(torch.int32)
+            P.table[:, :-1] = order[:n * (P.table.shape[1] - 1)].view(n, -1)
+            P.k.copy_(half(g, *P.k.shape))
+            P.v.copy_(half(g, *P.v.shape))
+            st["lens"].copy_(ints(lens))
+            st["qkv"].copy_(half(g, *st["qkv"].shape))
+            st["q"].fill_(float("nan"))
+            st["out"].fill_(float("nan"))
+            want_v, want_k = P.v.clone(), P.k.double()
+            tol_k = torch.zeros_like(want_k)
+            graph.replay()
+            torch.cuda.synchronize()
+            kernels.device_status()
+            q, k, v = st["qkv"].split([H, Hk, Hk], 1)
+            for s in range(n):
+                rows, pos = slice(s * m, (s + 1) * m), torch.arange(lens[s] - m, lens[s], device="cuda")
+                assert_close(st["q"][rows], *rotate(q[rows], pos, hd, 10000.0, False, RopeScaling()), "q")
+                at = P.table[s].long()[pos // page], pos % page
+                want_k[at], tol_k[at] = rotate(k[rows], pos, hd, 10000.0, False, RopeScaling())
+                want_v[at] = v[rows]
+            assert_close(P.k, want_k, tol_k, "k")
+            assert torch.equal(P.v, want_v)
+            for s in range(n):
+                keys, values = (positions_of(t, P.table[s], lens[s]) for t in (P.k, P.v))
+                rows = slice(s * m, (s + 1) * m)
+                assert_close(st["out"][rows], *attend(st["q"][rows], keys, values, 0.1, lens[s] - m + 1), s)
+    finally:
+        kernels.set_tunable("pdl", 0)
+
+
+def test_many_calls_on_two_streams(kernels):
+    """Both streams are kept busy, with a workspace each and an output for each call: every one of them is right."""
+    jobs = []
+    for i, (H, Hk, hd, new, lens) in enumerate([(32, 8, 128, [1] * 6, [3000, 10, 500, 1500, 64, 2000]),
+                                                (16, 16, 64, [40, 1, 9], [2500, 700, 9])]):
+        q, P, kv, cu = paged_case(new, lens, H, Hk, hd, 32, "tokens", seed=i, spare=0)
+        outs = [torch.full_like(q, float("nan")) for _ in range(12)]
+        jobs.append((torch.cuda.Stream(), q, P, kv, new, lens, ints(cu), ints(lens), outs,
+                     kernels.attention_paged_workspace(H, Hk, hd)))
+    torch.cuda.synchronize()
+    for r in range(12):
+        for stream, q, P, kv, new, lens, cu, n, outs, ws in jobs:
+            kernels.attention_paged(view(outs[r]), view(q), P.k, P.v, P.table, cu, n, max(new), 0.1, ws, stream=stream)
+    torch.cuda.synchronize()
+    kernels.device_status()
+    for stream, q, P, kv, new, lens, cu, n, outs, ws in jobs:
+        at = starts(new)
+        for s in range(len(new)):
+            rows = slice(at[s], at[s + 1])
+            assert_close(outs[0][rows], *attend(q[rows], *kv[s], 0.1, lens[s] - new[s] + 1), s)
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
 @pytest.mark.parametrize("paged", [True, False])
 @pytest.mark.parametrize("n,T,H,Hk,hd", [(64, 2048, 32, 8, 64), (31, 2048, 8, 8, 128), (200, 300, 4, 4, 64), (9, 130, 2, 1, 128)])
 def test_tiles_of_overlapping_sequences(kernels, paged, n, T, H, Hk, hd):
