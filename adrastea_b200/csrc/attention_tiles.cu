@@ -13,6 +13,9 @@
 //   * the maximum m that a row is scaled by is moved only when a score passes it by more than 2^8: the rescaling of O in
 //     tensor memory is rare.  P and the sums are carried times 2^7, so that they end at 2^15, within fp16's range, and what
 //     is small keeps as many bits as there are: 11 down to 2^-21 of a row's largest weight, 2^-32 of it below;
+//   * the tensor cores' sums round towards zero, 1e-7 of a sum for every 16 products (values of one sign were off by 8.4e-4
+//     after 131072 keys, by 7e-3 after a million): every 32768 keys, where that is 2^-12 of the sum, the softmax warps take out
+//     of O what a row's mean so far stands for, and the sum begins anew;
 //   * when S of a block is complete, so is the product with V before it (the tensor cores run in order), so the softmax
 //     warps may touch O and no further barrier is needed;
 //   * few tiles over many pages: the keys of each are shared out among CTAs, and a second kernel joins the parts.
@@ -45,6 +48,9 @@ constexpr float TL_FAR = 0x1p20f;
 __device__ __forceinline__ bool is_far(float base) {  // (not infinity, nor what is not a number)
   return __float_as_uint(fabsf(base)) - __float_as_uint(TL_FAR) < 0x7F800000u - __float_as_uint(TL_FAR);
 }
+// Keys after which the sum in O begins anew (2048 sums of 16 products lose 2e-4 of what they begin from zero), in kernels of
+// their own: with that code 32 x 257 tokens took 41.9 instead of 39.2 us, 4 chunks of 512 over up to 16384 295 instead of 281.
+constexpr int TL_LONG = 32768;
 // Of every eight pairs of probabilities, those that the FMA units compute; the others go to the exponential unit.
 constexpr int BY_FMA = 1;
 
@@ -246,7 +252,37 @@ __device__ __forceinline__ bool tile_any(int tile, bool x) {
   return r != 0;
 }
 
-template <int HD, int NT, int N, bool PAGED, bool SPLIT>
+// Eight columns of a row's mean, which stand for what has been taken out of the sum in O: kept where the row's output goes
+// (16-bit, and zeros where it would not be finite), or its part (32-bit).  `o` comes back as what is left of the sum.
+template <bool SPLIT>
+__device__ __forceinline__ void add_mean(const uint8_t* at, float weight, uint32_t* o) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 x = SPLIT ? reinterpret_cast<const float2*>(at)[i / 2] : __half22float2(reinterpret_cast<const __half2*>(at)[i / 2]);
+    o[i] = __float_as_uint(fmaf(weight, x.x, __uint_as_float(o[i])));
+    o[i + 1] = __float_as_uint(fmaf(weight, x.y, __uint_as_float(o[i + 1])));
+  }
+}
+template <bool SPLIT>
+__device__ __forceinline__ void take_mean(uint8_t* at, float l, float inv, uint32_t* o) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float2 x = make_float2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+    if (!(fabsf(x.x) <= 65504.0f)) x.x = 0.0f;
+    if (!(fabsf(x.y) <= 65504.0f)) x.y = 0.0f;
+    if constexpr (SPLIT) {
+      reinterpret_cast<float2*>(at)[i / 2] = x;
+    } else {
+      const __half2 h = __floats2half2_rn(x.x, x.y);
+      reinterpret_cast<__half2*>(at)[i / 2] = h;
+      x = __half22float2(h);
+    }
+    o[i] = __float_as_uint(fmaf(-l, x.x, __uint_as_float(o[i])));
+    o[i + 1] = __float_as_uint(fmaf(-l, x.y, __uint_as_float(o[i + 1])));
+  }
+}
+
+template <int HD, int NT, int N, bool PAGED, bool SPLIT, bool LONG>
 __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N>::CTAS)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TileParams p) {
@@ -265,6 +301,7 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + SLOTS);
   volatile uint32_t* by_hand = tmem_slot + 1;  // [NT] the softmax warps did this block's product with V
   __shared__ TileJob s_job;
+  __shared__ float s_mean[LONG ? NT * TL_M : 1];  // the sum of probabilities that a row's mean (see take_mean) stands for
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr bool ONE = Cfg::ONE;
@@ -573,6 +610,17 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
 
+    // where the row's output goes, or its part; computed anew (the compiler would hold it in registers through the loop)
+    auto row_at = [&]() -> uint8_t* {
+      int r = row;
+      asm volatile("" : "+r"(r));
+      if constexpr (SPLIT) return reinterpret_cast<uint8_t*>(p.part_o + ((size_t)blockIdx.x * TL_M + r) * HD);
+      const int tk = r / p.a.group;
+      return reinterpret_cast<uint8_t*>(p.a.out + (long long)(span.q0 + first + tk) * p.a.so[0] +
+                                        (long long)(head * p.a.group + r - tk * p.a.group) * p.a.so[1]);
+    };
+    constexpr int MEAN = SPLIT ? 4 : 2;  // bytes of a column there
+    constexpr int FOLD = TL_LONG / N;
     const uint32_t b_s = smem_u32(&s_ready[t]), b_p = smem_u32(&p_ready[t]), b_h = smem_u32(&p_half[t]);
     for (int j = 0; j < my_nb; ++j) {
       const int key0 = (j0 + j) * N;
@@ -655,7 +703,8 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
         // it matters; a sum with the slack would round it away in large maxima.)
         const bool move = mx - m > slack;
         float base = m * scale2;
-        if (__any_sync(0xffffffffu, move || is_far(base))) {
+        const bool fold = LONG && j % FOLD == 0 && j > 0;
+        if (__any_sync(0xffffffffu, move || fold || is_far(base))) {
           const float alpha = move ? (m == -INFINITY ? 0.0f : exp2_fast((m - mx) * scale2)) : 1.0f;
           if (move) m = mx;
           l *= alpha;
@@ -669,6 +718,25 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
               for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
               tmem_st_x8(o_at + c, o);
             }
+            if (LONG && j > FOLD) s_mean[t * TL_M + row] *= alpha;
+          }
+          if (fold) {
+            const float weight = j > FOLD ? s_mean[t * TL_M + row] : 0.0f, inv = 1.0f / l;
+            uint8_t* at = row_at();
+            tmem_wait_st();
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 8, at += 8 * MEAN) {
+              uint32_t o[8];
+              tmem_ld_x8(o_at + c, o);
+              tmem_ld_wait();
+              if (live) {
+                if (j > FOLD) add_mean<SPLIT>(at, weight, o);
+                take_mean<SPLIT>(at, l, inv, o);
+              }
+              __syncwarp();
+              tmem_st_x8(o_at + c, o);
+            }
+            s_mean[t * TL_M + row] = l;
           }
           base = m * scale2;
           if (__any_sync(0xffffffffu, is_far(base))) {
@@ -805,12 +873,19 @@ __global__ void __launch_bounds__(TileCfg<HD, NT, N>::THREADS, TileCfg<HD, NT, N
       const float inv = limit > 0 ? 1.0f / (m == -INFINITY ? 0.0f : l) : 0.0f;
       __half* dst = p.a.out + (long long)(span.q0 + first + tok) * p.a.so[0] +
                     (long long)(head * p.a.group + row - tok * p.a.group) * p.a.so[1];
+      const bool folded = LONG && my_nb > FOLD;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
         if (my_nb > 0) {
           tmem_ld_x32(o_at + c, o);
           tmem_ld_wait();
+        }
+        if (folded && live) {
+          const float weight = s_mean[t * TL_M + row];
+          const uint8_t* at = row_at() + c * MEAN;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) add_mean<SPLIT>(at + i * MEAN, weight, o + i);
         }
         if (SPLIT && live && my_nb > 0) {
           float4* to = reinterpret_cast<float4*>(p.part_o + ((size_t)blockIdx.x * TL_M + row) * HD + c);
@@ -918,11 +993,11 @@ long long most_jobs(const SeqAttention& a, int nt) {
   return std::min<long long>(a.tokens, (a.tokens + a.n_seqs * (per - 1)) / per) * a.n_kv_heads;
 }
 
-template <int HD, int NT, int N, bool PAGED, bool SPLIT>
+template <int HD, int NT, int N, bool PAGED, bool SPLIT, bool LONG>
 int launch_tiles_as(adr_ctx* ctx, cudaStream_t stream, const SeqAttention& a, int min_rows, int splits = 1,
                     uint8_t* workspace = nullptr) {
   using Cfg = TileCfg<HD, NT, N>;
-  auto kfn = attention_tiles_kernel<HD, NT, N, PAGED, SPLIT>;
+  auto kfn = attention_tiles_kernel<HD, NT, N, PAGED, SPLIT, LONG>;
   if (int rc = opt_in_smem(ctx, kfn, Cfg::SMEM); rc != ADR_OK) return rc;
   TileParams p = {};
   p.a = a;
@@ -981,22 +1056,35 @@ int launch_attention_tiles(adr_ctx* ctx, cudaStream_t stream, const SeqAttention
   // causal: 4 x 2048 tokens (1024 tiles) 93 against 78 us, 16 x 512 (1024) 39 against 39; all keys seen: 16 x 512 36 against
   // 42, 4 x 2048 107 against 120; 32/32 heads, causal: 1 x 2048 (512 tiles) 46 against 42, 2 x 8192 (4096) 749 against 813.
   if (a.block_table == nullptr) {
-    const long long jobs = most_jobs(a, 1);
-    if (a.head_dim == 64)
-      return jobs > (a.causal && max_q > 512 ? 4 : 2) * tile_parts(ctx)
-                 ? launch_tiles_as<64, 1, 64, false, false>(ctx, stream, a, min_rows)
-                 : launch_tiles_as<64, 1, 128, false, false>(ctx, stream, a, min_rows);
-    return max_q <= 2048 ? launch_tiles_as<128, 1, 128, false, false>(ctx, stream, a, min_rows)
-                         : launch_tiles_as<128, 2, 128, false, false>(ctx, stream, a, min_rows);
+    const bool many_keys = max_q > TL_LONG;
+    if (a.head_dim == 64) {
+      if (most_jobs(a, 1) > (a.causal && max_q > 512 ? 4 : 2) * tile_parts(ctx))
+        return many_keys ? launch_tiles_as<64, 1, 64, false, false, true>(ctx, stream, a, min_rows)
+                         : launch_tiles_as<64, 1, 64, false, false, false>(ctx, stream, a, min_rows);
+      return many_keys ? launch_tiles_as<64, 1, 128, false, false, true>(ctx, stream, a, min_rows)
+                       : launch_tiles_as<64, 1, 128, false, false, false>(ctx, stream, a, min_rows);
+    }
+    if (many_keys) return launch_tiles_as<128, 2, 128, false, false, true>(ctx, stream, a, min_rows);
+    return max_q <= 2048 ? launch_tiles_as<128, 1, 128, false, false, false>(ctx, stream, a, min_rows)
+                         : launch_tiles_as<128, 2, 128, false, false, false>(ctx, stream, a, min_rows);
   }
   const int splits = attention_tiles_splits(ctx, a);
-  if (splits > 1)
-    return a.head_dim == 64 ? launch_tiles_as<64, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace)
-                            : launch_tiles_as<128, 1, 128, true, true>(ctx, stream, a, min_rows, splits, (uint8_t*)workspace);
-  if (a.head_dim == 64) return launch_tiles_as<64, 1, 128, true, false>(ctx, stream, a, min_rows);
-  return (long long)a.max_pages * a.page_size <= 512
-             ? launch_tiles_as<128, 1, 128, true, false>(ctx, stream, a, min_rows)
-             : launch_tiles_as<128, 2, 128, true, false>(ctx, stream, a, min_rows);
+  const long long keys = (long long)a.max_pages * a.page_size;
+  const bool many_keys = keys > (long long)splits * TL_LONG;
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  if (splits > 1) {
+    if (a.head_dim == 64)
+      return many_keys ? launch_tiles_as<64, 1, 128, true, true, true>(ctx, stream, a, min_rows, splits, ws)
+                       : launch_tiles_as<64, 1, 128, true, true, false>(ctx, stream, a, min_rows, splits, ws);
+    return many_keys ? launch_tiles_as<128, 1, 128, true, true, true>(ctx, stream, a, min_rows, splits, ws)
+                     : launch_tiles_as<128, 1, 128, true, true, false>(ctx, stream, a, min_rows, splits, ws);
+  }
+  if (a.head_dim == 64)
+    return many_keys ? launch_tiles_as<64, 1, 128, true, false, true>(ctx, stream, a, min_rows)
+                     : launch_tiles_as<64, 1, 128, true, false, false>(ctx, stream, a, min_rows);
+  if (many_keys) return launch_tiles_as<128, 2, 128, true, false, true>(ctx, stream, a, min_rows);
+  return keys <= 512 ? launch_tiles_as<128, 1, 128, true, false, false>(ctx, stream, a, min_rows)
+                     : launch_tiles_as<128, 2, 128, true, false, false>(ctx, stream, a, min_rows);
 }
 
 }  // namespace adr

@@ -1,0 +1,132 @@
+"""Attention over so many keys that the tensor cores' sums, which round towards zero, would drift: sums, maxima that move, and
+what is not finite, over more than 32768 keys, in every form of tile."""
+import pytest
+import torch
+
+from adrastea_b200 import MatmulMask
+from serving_oracle import assert_close, attend
+from test_gpu_serving import gen, half, ints, view
+
+pytestmark = pytest.mark.gpu
+PAGE = 256
+INF, NAN = float("inf"), float("nan")
+
+
+def run(kernels, kind, q, k, v, scale, hint=None, spare=5):
+    """One causal sequence: q [new, H, hd], k and v [n, Hk, hd], n a multiple of PAGE where `kind` is paged; `spare` rows of no
+    sequence behind it are left alone."""
+    new, H, hd = q.shape
+    n, Hk = k.shape[:2]
+    rows = torch.cat([q, q.new_full((spare, H, hd), NAN)])
+    out = torch.full_like(rows, 3.0)
+    if kind == "packed":
+        k, v = (torch.cat([t, t.new_full((spare, Hk, hd), NAN)]) for t in (k, v))
+        kernels.attention_packed(view(out), view(rows), view(k), view(v), ints([0, n]), hint or n, scale, MatmulMask.Causal)
+    else:
+        table = torch.arange(n // PAGE, dtype=torch.int32, device="cuda")[None].contiguous()
+        pool = [t.view(n // PAGE, PAGE, Hk, hd) for t in (k, v)]
+        kernels.attention_paged(view(out), view(rows), *pool, table, ints([0, new]), ints([n]), hint or new, scale,
+                                kernels.attention_paged_workspace(H, Hk, hd))
+    kernels.device_status()
+    assert (out[new:] == 3.0).all()
+    return out[:new]
+
+
+# how it is called, new rows, positions, query heads, key heads, head_dim, max_q if not the rows
+FAR = [("paged", 300, 1 << 19, 64, 1, 128, None), ("paged", 300, 1 << 19, 64, 1, 64, None),
+       ("paged", 296, 1 << 21, 64, 1, 64, None), ("paged", 296, 1 << 21, 64, 1, 128, None),  # keys shared by two CTAs
+       ("packed", 1 << 17, 1 << 17, 1, 1, 64, None), ("packed", 1 << 18, 1 << 18, 1, 1, 64, None),
+       ("packed", 1 << 18, 1 << 18, 1, 1, 128, None)]
+
+
+@pytest.mark.parametrize("kind,new,n,H,Hk,hd,hint", FAR)
+def test_sums_over_many_keys_do_not_drift(kernels, kind, new, n, H, Hk, hd, hint):
+    """Equal weights, which fp16 holds, and values of one sign: a mean.
+
+    Bound: the output's rounding, 2^-11, and what is dropped within 32768 keys: 2048 sums of 16 products, which lose 2^-23 of
+    what has been summed each."""
+    g = gen(n + hd)
+    q, k = torch.zeros((new, H, hd), dtype=torch.float16, device="cuda"), half(g, n, Hk, hd)
+    v = (1 + torch.rand((n, Hk, hd), device="cuda", generator=g)).half()
+    out = run(kernels, kind, q, k, v, 0.1, hint)
+    for i in (0, 1, new // 3, new // 2, new - 2, new - 1):
+        seen = n - new + i + 1
+        want = v[:seen, 0].double().mean(0).expand(H, hd)
+        assert_close(out[i], want, want * (2.0 ** -11 + 2.0 ** -12), i)
+
+
+MOVES = [("paged", 300, 81920, 64, 1, 128, None), ("paged", 300, 81920, 64, 1, 64, None), ("paged", 298, 1 << 17, 64, 1, 64, None),
+         ("paged", 148, 1 << 17, 128, 2, 128, None), ("paged", 148, 1 << 17, 128, 2, 64, None),
+         ("packed", 70000, 70000, 2, 1, 64, None), ("packed", 70000, 70000, 4, 4, 64, None), ("packed", 70000, 70000, 2, 1, 128, None)]
+
+
+def some_rows(new):
+    return sorted({0, 1, new // 7, new // 2, new - 1} | {r for r in (8191, 8192, 8300, 12289, 32767, 32768, 33000, 66000) if r < new})
+
+
+@pytest.mark.parametrize("kind,new,n,H,Hk,hd,hint", MOVES)
+@pytest.mark.parametrize("shape", ["grow", "fall", "waves", "far", "minus"])
+def test_maxima_that_move_over_many_keys(kernels, kind, new, n, H, Hk, hd, hint, shape):
+    """Scores that grow by 60 over the keys (every part of the sum counts less and less), fall, rise and fall again; maxima of
+    4 million; scores of -infinity up to the middle.  The oracle's bound, with 2^-12 of the weighted values' sizes for the sums
+    (see above)."""
+    g = gen(n + H)
+    at = torch.linspace(0, 1, n, device="cuda")
+    ramp = {"grow": 60 * at, "fall": -60 * at, "waves": 20 * torch.sin(at * 40) + 20 * at, "far": 60 * at,
+            "minus": torch.where(at < 0.5, -INF, 10 * at)}[shape]
+    q, k = 0.1 * half(g, new, H, hd), half(g, n, Hk, hd)
+    q[..., 0], k[..., 0] = 1.0, ramp.half()[:, None]
+    v = (0.5 + torch.rand((n, Hk, hd), device="cuda", generator=g)).half()
+    scale = 1.0
+    if shape == "far":   # every score of the ramp, a step of 512 apart
+        q[..., 1:] = 0
+        q[..., 0], k[..., 0] = 4096.0, (torch.floor(ramp * 16)).half()[:, None]
+    out = run(kernels, kind, q, k, v, scale, hint)
+    for i in some_rows(new):
+        seen = n - new + i + 1
+        first = int((at < 0.5).sum()) if shape == "minus" else 0   # (what is before has no weight)
+        for h in {0, H - 1}:
+            if seen <= first:
+                assert out[i, h].isnan().all()
+                continue
+            kk, vv = k[first:seen, h // (H // Hk)][:, None], v[first:seen, h // (H // Hk)][:, None]
+            want, tol = attend(q[i:i + 1, h:h + 1], kk, vv, scale, seen - first)
+            assert_close(out[i:i + 1, h:h + 1], want, tol + want.abs() * 2.0 ** -12, (i, h))
+
+
+@pytest.mark.parametrize("kind,new,n,H,Hk,hd,hint", MOVES)
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_a_bad_value_among_many(kernels, kind, new, n, H, Hk, hd, hint, value):
+    """One token's value is not finite in one column: the rows before it, and the other columns, do not see it."""
+    for at in {100, n - new // 2, n - 1} if kind == "packed" else {100, n // 2, n - new // 2}:
+        g = gen(n + H + at)
+        q, k = half(g, new, H, hd), half(g, n, Hk, hd)
+        v = (0.5 + torch.rand((n, Hk, hd), device="cuda", generator=g)).half()
+        clean = run(kernels, kind, q, k, v, 0.1, hint)
+        v[at, :, 3] = value
+        out = run(kernels, kind, q, k, v, 0.1, hint)
+        first = max(0, at - (n - new))
+        # (rows that share a block with it may be summed in another order: 2^-22 of the 128 weights and more; fp16 rounds both)
+        same = torch.isclose(out.float(), clean.float(), rtol=2.0 ** -10, atol=2.0 ** -14)
+        assert same[:first].all(), at
+        assert same[..., 4:].all() and same[..., :3].all(), at
+        assert not out[first:, :, 3].isfinite().any(), at
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,Hk", [(2, 2), (64, 1)])
+def test_more_rows_than_positions(kernels, hd, H, Hk):
+    """The first rows lie before position 0 and are zeros, in a sequence of many positions all the same."""
+    new, n = 50000, 40000
+    g = gen(hd + H)
+    q, k, v = half(g, new, H, hd), half(g, n, Hk, hd), half(g, n, Hk, hd)
+    out = torch.full_like(q, NAN)
+    table = torch.arange(n // 64, dtype=torch.int32, device="cuda")[None].contiguous()
+    kernels.attention_paged(view(out), view(q), k.view(n // 64, 64, Hk, hd), v.view(n // 64, 64, Hk, hd), table, ints([0, new]),
+                            ints([n]), new, 0.1, kernels.attention_paged_workspace(H, Hk, hd))
+    kernels.device_status()
+    assert not out[:new - n].any()
+    for i in (new - n, new - n + 1, new - 3000, new - 1):
+        seen = n - new + i + 1
+        want, tol = attend(q[i:i + 1, :1], k[:seen, :1], v[:seen, :1], 0.1, seen)
+        assert_close(out[i:i + 1, :1], want, tol + 2.0 ** -12, i)
