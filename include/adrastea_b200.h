@@ -576,7 +576,7 @@ int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_out, const vo
  * rows of k and v, mask Causal hiding key x from row y when x > y.  Scores, maxima and sums are fp32
  * (scale is not rounded), probabilities are rounded to fp16 for the product with v (2^-11 of each, or
  * 2^-32 of the row's largest where that is more), the output once.  The sums over keys round towards
- * zero, by 2^-12 of what is summed at most.  `max_q`: the longest sequence's rows; it chooses the
+ * zero, by about 2^-12 of what is summed at most.  `max_q`: the longest sequence's rows; it chooses the
  * kernel and does not change what is computed (but for that bound, which does not hold for sequences
  * of more than 32768 rows where max_q says that there are none).  head_dim 64 or 128, n_heads a
  * multiple of n_kv_heads and at most 64 times it, pointers 16-byte aligned, strides of dimensions of

@@ -130,3 +130,66 @@ def test_more_rows_than_positions(kernels, hd, H, Hk):
         seen = n - new + i + 1
         want, tol = attend(q[i:i + 1, :1], k[:seen, :1], v[:seen, :1], 0.1, seen)
         assert_close(out[i:i + 1, :1], want, tol + 2.0 ** -12, i)
+
+
+# ------------------------------------------------------------------ a few rows
+# sequences, new rows, positions, query heads, key heads, head_dim: whole sequences to a CTA
+FEW = [(40, 1, 1 << 20, 8, 8, 64), (40, 1, 1 << 20, 8, 8, 128), (40, 1, 1 << 20, 64, 8, 64), (20, 1, 1 << 20, 128, 8, 128),
+       (40, 5, 1 << 20, 32, 8, 128), (40, 20, 1 << 20, 8, 8, 64), (3, 1, 1 << 20, 4, 2, 128)]
+
+
+def few(kernels, q, k, v, S, scale, new):
+    """`S` sequences that share all their pages."""
+    n, Hk, hd = k.shape
+    H = q.shape[1]
+    table = torch.arange(n // PAGE, dtype=torch.int32, device="cuda")[None].expand(S, -1).contiguous()
+    pool = [t.view(n // PAGE, PAGE, Hk, hd) for t in (k, v)]
+    out = torch.full((S * new + 3, H, hd), 3.0, dtype=torch.float16, device="cuda")
+    rows = torch.cat([q, q.new_full((3, H, hd), NAN)])
+    kernels.attention_paged(view(out), view(rows), *pool, table, ints([i * new for i in range(S + 1)]), ints([n] * S), new, scale,
+                            kernels.attention_paged_workspace(H, Hk, hd))
+    kernels.device_status()
+    assert (out[S * new:] == 3.0).all()
+    return out[:S * new]
+
+
+@pytest.mark.parametrize("S,new,n,H,Hk,hd", FEW)
+def test_sums_of_few_rows_do_not_drift(kernels, S, new, n, H, Hk, hd):
+    """As above, with 32768 keys to a warp between two beginnings."""
+    g = gen(n + hd)
+    q, k = torch.zeros((S * new, H, hd), dtype=torch.float16, device="cuda"), half(g, n, Hk, hd)
+    v = (1 + torch.rand((n, Hk, hd), device="cuda", generator=g)).half()
+    out = few(kernels, q, k, v, S, 0.1, new)
+    want = v.double().mean(0).repeat_interleave(H // Hk, 0)
+    # (an earlier row sees up to 19 keys fewer of a million, whose mean differs by less than 2^-15)
+    assert_close(out, want.expand(S * new, H, hd), (want * (2.0 ** -11 + 2.0 ** -12) + 2.0 ** -15).expand(S * new, H, hd))
+
+
+@pytest.mark.parametrize("S,new,n,H,Hk,hd", FEW)
+@pytest.mark.parametrize("shape", ["grow", "fall", "waves", "minus", "nan", "inf"])
+def test_maxima_of_few_rows_that_move(kernels, S, new, n, H, Hk, hd, shape):
+    """Scores that grow over the keys, fall, rise and fall again; that are -infinity up to the middle; a value that is not
+    finite, which every row sees: other columns do not."""
+    n = 300 * 1024
+    g = gen(n + H)
+    at = torch.linspace(0, 1, n, device="cuda")
+    ramp = {"grow": 40 * at, "fall": -40 * at, "waves": 15 * torch.sin(at * 40) + 15 * at,
+            "minus": torch.where(at < 0.5, -INF, 10 * at)}.get(shape, 0 * at)
+    q, k = 0.1 * half(g, S * new, H, hd), half(g, n, Hk, hd)
+    q[..., 0], k[..., 0] = 1.0, ramp.half()[:, None]
+    v = (0.5 + torch.rand((n, Hk, hd), device="cuda", generator=g)).half()
+    first = int((at < 0.5).sum()) if shape == "minus" else 0
+    clean = v.clone()
+    if shape in ("nan", "inf"):
+        v[1000, :, 3] = NAN if shape == "nan" else INF
+    out = few(kernels, q, k, v, S, 1.0, new)
+    if shape in ("nan", "inf"):
+        assert not out[..., 3].isfinite().any()
+        out[..., 3] = 0
+        clean[..., 3] = 0
+    for i in sorted({0, new - 1, S * new // 2, S * new - 1}):
+        seen = n - new + i % new + 1
+        for h in {0, H - 1}:
+            kk, vv = k[first:seen, h // (H // Hk)][:, None], clean[first:seen, h // (H // Hk)][:, None]
+            want, tol = attend(q[i:i + 1, h:h + 1], kk, vv, 1.0, seen - first)
+            assert_close(out[i:i + 1, h:h + 1], want, tol + want.abs() * 2.0 ** -12, (i, h))
