@@ -497,7 +497,9 @@ class LlamaU8:
         cu_q, before = ints(starts), list(cache.length)
         cache.extend(seqs, new)
         try:
-            kv_len, table = ints([cache.length[s] for s in seqs]), cache.table[seqs]
+            lens = [cache.length[s] for s in seqs]
+            # (as wide as the longest sequence: the attention chooses its kernels by what the table may hold)
+            kv_len, table = ints(lens), cache.table[seqs, :-(-max(lens) // cache.page_size)]
             for li, ly in enumerate(self.layers):
                 self._norm(x, h, ly.attn_norm)
                 self._prefill_linear(ly.wqkv, qkv, x)

@@ -594,7 +594,9 @@ int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, const void*
  * Arithmetic, max_q and rules as in adr_attention_packed; page_size a power of two from 16 to 256.
  * `workspace`: adr_attention_paged_workspace bytes of device memory, 16-byte aligned, whatever they
  * hold.  Calls that overlap in time need one each.  `max_q` should be the largest lq: it chooses
- * between a kernel of up to 32 rows of a key head and one of tiles of 128.
+ * between a kernel of up to 32 rows of a key head and one of tiles of 128.  `max_pages` should be what
+ * the longest sequence needs: over how many CTAs a tile's keys are spread, and which form of a kernel
+ * runs, is chosen by the positions that the table may hold, since the lengths are device memory.
  */
 size_t adr_attention_paged_workspace(const adr_ctx* ctx, int n_heads, int n_kv_heads, int head_dim);
 int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, const void* q, const void* k_pages,

@@ -87,6 +87,17 @@ def test_truncated_sequences_give_back_the_pages_behind_their_end():
         c.truncate(2, 0)
 
 
+def test_a_step_hands_over_as_much_of_the_table_as_it_needs():
+    """The attention chooses its kernels by the table's width: a short batch in a cache for long sequences is a short one."""
+    m = model()
+    c = m.paged_cache(pages=9, page_size=16, max_positions=4096)
+    for seqs, toks, columns in (([0], [20], 2), ([2, 0], [3, 13], 3), ([2], [13], 1), ([1, 2], [1, 1], 2)):
+        m.extend(c, seqs, [torch.arange(n) for n in toks])
+        for call in (m.k.rope_append_paged.call_args, m.k.attention_paged.call_args):
+            table = next(a for a in call.args if torch.is_tensor(a) and a.dim() == 2 and a.dtype == torch.int32)
+            assert table.is_contiguous() and torch.equal(table, c.table[seqs][:, :columns])
+
+
 # ------------------------------------------------------------------ sizes
 MANY = 1 << 32   # C's int would make 0 of it, and of MANY + 5 five
 
