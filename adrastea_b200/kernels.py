@@ -845,6 +845,8 @@ class GpuKernels:
     def attention_paged_workspace(self, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor:
         """A workspace for attention_paged of these heads.  Calls that overlap in time need one each."""
         need = self._lib.adr_attention_paged_workspace(self._ctx, n_heads, n_kv_heads, head_dim)
+        if need == 0:  # (an empty workspace would be refused later, and for another reason)
+            self._check(2)
         return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", self.device))
 
     def attention_paged(self, out: TensorView, q: TensorView, k_pages: torch.Tensor, v_pages: torch.Tensor,

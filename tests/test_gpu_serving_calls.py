@@ -213,3 +213,10 @@ def test_a_step_that_fails_is_as_if_it_had_not_been(kernels, monkeypatch):
         model.extend(rough, seqs, t)
         assert torch.equal(model.logits, w)
     kernels.device_status()
+
+
+@pytest.mark.parametrize("H,Hk,hd", [(8, 2, 96), (8, 3, 64), (130, 2, 64), (0, 1, 64), (4, -1, 64)])
+def test_a_workspace_of_heads_that_are_not_taken_is_refused(kernels, H, Hk, hd):
+    with pytest.raises(AdrError) as e:
+        kernels.attention_paged_workspace(H, Hk, hd)
+    assert e.value.code == 2
