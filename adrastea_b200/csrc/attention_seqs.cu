@@ -11,12 +11,13 @@ namespace adr {
 namespace {
 
 // Rows of a key head up to which the kernel of few rows takes a sequence.  (32 rows over 32768 positions: 38 against 85 us
-// in tiles, 32 x 1000: 46 against 40; from 40 rows on the tiles are ahead nearly everywhere, 32 x 1000: 160 against 143.)
+// in tiles, 32 x 1000: 46 against 40; from 40 rows on the tiles are ahead nearly everywhere, 32 x 1000: 160 against 143.  Fitted to
+// head_dim 128: of 64, 32 x 1000 takes 31.5 us here and 18.7 in tiles.)
 constexpr int FEW_ROWS = 32;
 
 // Keys of a tile's part up to which a second kernel for the sequences of few rows costs more than their tiles (6 sequences of
 // up to 100 tokens over up to 4096 positions, 32/8 heads: 43 against 56 us; a single token's tile over more would be what all
-// others wait for).
+// others wait for).  By the table's width, as the number of parts is: the figures are of tables as wide as the longest sequence.
 constexpr int ALONE_KEYS = 4096;
 
 // The strides of n dimensions of the given extents: not negative, and 16-byte steps where a dimension has more

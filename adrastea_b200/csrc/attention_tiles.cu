@@ -20,9 +20,9 @@
 //     warps may touch O and no further barrier is needed;
 //   * few tiles over many pages: the keys of each are shared out among CTAs, and a second kernel joins the parts.
 // What bounds it: no unit alone.  Two prompts of 8192 tokens, 64/8 heads of 128: 1.9 ms, 1160 TFLOP/s of 1625 in short runs
-// and 2.2 to 2.3 ms at the power limit, where the clock falls to 1.63 GHz; the tensor cores are busy for half of the time, the
+// and 2.2 to 2.3 ms at the power limit, where the clock falls to 1.62 GHz; the tensor cores are busy for half of the time, the
 // exponential unit for 43 %, issue slots for 36 % (2 x 4096 tokens, 32/8 heads), each softmax pass waiting for the product
-// before it.  Of 257 tokens and head_dim 64 (images): 38 us where memory wants 10: each CTA begins and ends in about 5
+// before it.  Of 257 tokens and head_dim 64 (images): 39 us where memory wants 10: each CTA begins and ends in about 5
 // us of latency, a third of which the other three hide, and every third tile has one row.
 // What a causal row does not see must not reach it even if it is infinite or not a number; a probability of zero does
 // not see to that.  Keys are masked by selection.  Values behind the sequence's end are cleared in shared memory; a

@@ -3,8 +3,8 @@
 //
 // The angle of pair i at position p is p * f_i.  A 32-bit f_i would lose it at far positions (2^-24 relative of
 // 10^6 radians), and a 64-bit product costs the GPU's few fp64 units.  So the table holds f_i / (2 pi), the turns
-// per position, as a 64-bit fixed-point fraction; p times it modulo 2^64 is then the fraction of a turn, exact to
-// |p| * 2^-65, by integer multiplication, whatever the position's size or sign.  Its upper 32 bits become the
+// per position, as a 64-bit fixed-point fraction (cut off); p times it modulo 2^64 is then the fraction of a turn, off by
+// |p| * 2^-64 at most, by integer multiplication, whatever the position's size or sign.  Its upper 32 bits become the
 // argument of sincospif: what remains is the 2^-24 of a 32-bit float.
 #include <cmath>
 
