@@ -58,6 +58,7 @@ extern "C" int adr_attention_packed(adr_ctx* ctx, adr_stream stream, void* out, 
   if (int rc = check_steps(q, strides_q, 2, eq); rc != ADR_OK) return rc;
   if (int rc = check_steps(k, strides_k, 2, ek); rc != ADR_OK) return rc;
   if (int rc = check_steps(v, strides_v, 2, ek); rc != ADR_OK) return rc;
+  if (!on_elements(cu_q)) return ADR_ERR_SHAPE;
   if (!ctx) return ADR_ERR_INVALID;
   DeviceGuard guard(ctx);
   SeqAttention p = {};
@@ -108,7 +109,7 @@ extern "C" int adr_attention_paged(adr_ctx* ctx, adr_stream stream, void* out, c
   if (int rc = check_steps(q, strides_q, 2, eq); rc != ADR_OK) return rc;
   if (int rc = check_steps(k_pages, strides_kp, 3, ek); rc != ADR_OK) return rc;
   if (int rc = check_steps(v_pages, strides_vp, 3, ek); rc != ADR_OK) return rc;
-  if (reinterpret_cast<uintptr_t>(workspace) & 15u) return ADR_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) || !on_elements(block_table, cu_q, kv_len)) return ADR_ERR_SHAPE;
   if (!ctx) return ADR_ERR_INVALID;
   if (workspace_bytes < adr_attention_paged_workspace(ctx, n_heads, n_kv_heads, head_dim)) return ADR_ERR_SHAPE;
   DeviceGuard guard(ctx);

@@ -353,6 +353,7 @@ extern "C" int adr_rope_f16(adr_ctx* ctx, adr_stream stream, void* out, const vo
   if (int rc = check_rotation(turns, head_dim, rotary_dim, amplitude, layout); rc != ADR_OK) return rc;
   if (check_strides(strides_o, 2) != ADR_OK || check_strides(strides_i, 2) != ADR_OK) return ADR_ERR_INVALID;
   if ((long long)n_heads * head_dim > (1 << 30)) return ADR_ERR_SHAPE;
+  if (!on_elements((const __half*)out, (const __half*)in, positions, turns)) return ADR_ERR_SHAPE;
   if (!ctx) return ADR_ERR_INVALID;
   DeviceGuard guard(ctx);
   const bool vec = parts_in_pieces(head_dim, rotary_dim, layout) && in_pieces(out, strides_o, 2) &&
@@ -386,6 +387,9 @@ extern "C" int adr_rope_append_paged(adr_ctx* ctx, adr_stream stream, void* q_ou
     if (check_strides(s, 2) != ADR_OK) return ADR_ERR_INVALID;
   if (check_strides(strides_kp, 3) != ADR_OK || check_strides(strides_vp, 3) != ADR_OK) return ADR_ERR_INVALID;
   if (((long long)n_heads + n_kv_heads) * head_dim > (1 << 30)) return ADR_ERR_SHAPE;
+  if (!on_elements((const __half*)q_out, (const __half*)q, (const __half*)k, (const __half*)v, (const __half*)k_pages,
+                   (const __half*)v_pages, block_table, cu_q, kv_len, turns))
+    return ADR_ERR_SHAPE;
   if (!ctx) return ADR_ERR_INVALID;
   DeviceGuard guard(ctx);
   const bool vec = parts_in_pieces(head_dim, rotary_dim, layout) && in_pieces(q_out, strides_qo, 2) &&

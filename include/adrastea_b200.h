@@ -549,8 +549,8 @@ int adr_rope_turns(uint64_t* turns, float* amplitude, int rotary_dim, double the
  * adr_rotary for rows at any positions: rows of n_heads heads, pair (a, b) of row t becomes
  * amplitude * (a cos - b sin, b cos + a sin) of the angle positions[t] * f_i, in fp32 with one
  * rounding; columns from rotary_dim on are copied.  `turns` is device memory.  In place
- * (out == in with the same strides) is allowed.  Any strides and alignment; 16-byte pieces where
- * all rows, heads and parts of a head begin on one.  head_dim <= 256.
+ * (out == in with the same strides) is allowed.  Any strides, pointers to whole elements (else
+ * ADR_ERR_SHAPE); 16-byte pieces where all rows, heads and parts of a head begin on one.  head_dim <= 256.
  */
 int adr_rope_f16(adr_ctx* ctx, adr_stream stream, void* out, const void* in, int tokens, int n_heads,
                  int head_dim, const long long* strides_o, const long long* strides_i,

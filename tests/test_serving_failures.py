@@ -150,3 +150,27 @@ def test_a_table_of_another_size_is_refused(turns, rotary):
 
 def test_a_table_of_the_right_size_is_taken():
     assert RopeTable(torch.zeros(32, dtype=torch.int64), 64, RopeLayout.Half, 1.0).rotary_dim == 64
+
+
+# ------------------------------------------------------------------ alignment
+@pytest.mark.parametrize("name,change", [
+    ("rope_f16", dict(out=1)), ("rope_f16", dict(inp=3)), ("rope_f16", dict(positions=2)), ("rope_f16", dict(turns=4)),
+    ("rope_append_paged", dict(q_out=1)), ("rope_append_paged", dict(q=1)), ("rope_append_paged", dict(k=1)),
+    ("rope_append_paged", dict(v=1)), ("rope_append_paged", dict(kp=1)), ("rope_append_paged", dict(vp=1)),
+    ("rope_append_paged", dict(table=2)), ("rope_append_paged", dict(cu=1)), ("rope_append_paged", dict(lens=2)),
+    ("rope_append_paged", dict(turns=4)), ("attention_packed", dict(cu=2)), ("attention_paged", dict(table=2)),
+    ("attention_paged", dict(cu=2)), ("attention_paged", dict(lens=3))])
+def test_pointers_between_elements_are_refused(name, change):
+    """The GPU cannot read from there: the launch would end with a misaligned address."""
+    from test_serving_host import CALLS, _lib, _ptr
+    args = dict(CALLS[name], **{k: _ptr(offset) for k, offset in change.items()})
+    assert getattr(_lib.load(), "adr_" + name)(*args.values()) == 2
+
+
+@pytest.mark.parametrize("name", ["rope_f16", "rope_append_paged"])
+def test_pointers_to_any_element_are_taken(name):
+    """(As far as the missing context.)"""
+    from test_serving_host import CALLS, _lib, _ptr
+    halves = {"rope_f16": ("out", "inp"), "rope_append_paged": ("q_out", "q", "k", "v", "kp", "vp")}[name]
+    args = dict(CALLS[name], **{k: _ptr(2) for k in halves})
+    assert getattr(_lib.load(), "adr_" + name)(*args.values()) == 1
