@@ -193,3 +193,62 @@ def test_maxima_of_few_rows_that_move(kernels, S, new, n, H, Hk, hd, shape):
             kk, vv = k[first:seen, h // (H // Hk)][:, None], clean[first:seen, h // (H // Hk)][:, None]
             want, tol = attend(q[i:i + 1, h:h + 1], kk, vv, 1.0, seen - first)
             assert_close(out[i:i + 1, h:h + 1], want, tol + want.abs() * 2.0 ** -12, (i, h))
+
+
+# ------------------------------------------------------------------ long and short ones together
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("H,Hk", [(4, 2), (16, 16)])
+def test_long_and_short_prompts_together(kernels, hd, causal, H, Hk):
+    lens = [5, 70000, 300, 0, 40000, 129]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    g = gen(hd + H)
+    q, k = half(g, cu[-1] + 4, H, hd), half(g, cu[-1] + 4, Hk, hd)
+    v = (0.5 + torch.rand((cu[-1] + 4, Hk, hd), device="cuda", generator=g)).half()
+    for t in (q, k, v):
+        t[cu[-1]:] = NAN
+    out = torch.full_like(q, 3.0)
+    kernels.attention_packed(view(out), view(q), view(k), view(v), ints(cu), max(lens), 0.1,
+                             MatmulMask.Causal if causal else MatmulMask.None_)
+    kernels.device_status()
+    assert (out[cu[-1]:] == 3.0).all()
+    for s, n in enumerate(lens):
+        for i in sorted({0, n // 3, n - 1} | {r for r in (32767, 32768, 65600) if r < n}) if n else ():
+            for h in (0, H - 1):
+                seen = i + 1 if causal else n
+                rows, kh = slice(cu[s], cu[s] + seen), slice(h // (H // Hk), h // (H // Hk) + 1)
+                at = slice(cu[s] + i, cu[s] + i + 1)
+                want, tol = attend(q[at, h:h + 1], k[rows, kh], v[rows, kh], 0.1, seen)
+                assert_close(out[at, h:h + 1], want, tol + want.abs() * 2.0 ** -12, (s, i, h))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,Hk", [(8, 2), (64, 32)])
+@pytest.mark.parametrize("new,lens", [([300, 1, 40, 90], [100000, 120000, 50, 33000]), ([200] * 4, [90000, 200, 70000, 1000])])
+def test_chunks_and_tokens_over_long_and_short_caches(kernels, hd, H, Hk, new, lens):
+    g = gen(hd + H + new[1])
+    need = [-(-n // PAGE) for n in lens]
+    cu, first = [0], [0]
+    for m, pages in zip(new, need):
+        cu.append(cu[-1] + m)
+        first.append(first[-1] + pages)
+    pool_k = half(g, first[-1], PAGE, Hk, hd)
+    pool_v = (0.5 + torch.rand((first[-1], PAGE, Hk, hd), device="cuda", generator=g)).half()
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32, device="cuda")
+    for s, m in enumerate(need):
+        table[s, :m] = torch.arange(first[s], first[s + 1], device="cuda")
+    q = half(g, cu[-1], H, hd)
+    out, ws = torch.full_like(q, NAN), kernels.attention_paged_workspace(H, Hk, hd)
+    for _ in range(2):
+        kernels.attention_paged(view(out), view(q), pool_k, pool_v, table, ints(cu), ints(lens), max(new), 0.1, ws)
+    kernels.device_status()
+    for s, (m, n) in enumerate(zip(new, lens)):
+        keys, values = (t[first[s]:first[s + 1]].flatten(0, 1) for t in (pool_k, pool_v))
+        for i in sorted({0, m // 2, m - 1}):
+            for h in (0, H - 1):
+                seen, kh = n - m + i + 1, slice(h // (H // Hk), h // (H // Hk) + 1)
+                at = slice(cu[s] + i, cu[s] + i + 1)
+                want, tol = attend(q[at, h:h + 1], keys[:seen, kh], values[:seen, kh], 0.1, seen)
+                assert_close(out[at, h:h + 1], want, tol + want.abs() * 2.0 ** -12, (s, i, h))
